@@ -135,6 +135,60 @@ int b200gemm_k_grouped_static_scratch(const void* a, const void* b, void* c, con
                                       const int* group_start, const int* group_end, int num_groups, int64_t k_total,
                                       int m_dim, int n_dim, int dtype, int num_sms, void* stream);
 
+/* ---- gated feed-forward block of the experts, 16 bits --------------------------------------
+ * y = (act(x Wg_e^T) * (x Wu_e^T)) W2_e^T on rows grouped by expert.  The products whose epilogue is the
+ * gate are below; the others (y, dx, dW13, dW2) are b200gemm_m_grouped and b200gemm_k_grouped.  The
+ * reference leaves the activation to separate torch steps (README.md:175-179) and has no backward.
+ * act: 0 = silu, 1 = gelu (tanh form). */
+
+/* h [m_rows, inter] = act(g) * u with [g | u] = a w13_e^T, both products and the gate in one kernel; fp32
+ * accumulate, one rounding.  a [m_rows, k]; w13 [G, 2 inter, k]: gate rows, then up rows.
+ *   saved, saved_exps: NULL (inference), or both: g and u are kept for the gradient - saved
+ *   [m_rows, 2 inter] 16-bit codes and saved_exps, b200gemm_gated_exponent_bytes(m_rows, inter) bytes
+ *   (one power of two per 32 columns; the format is the library's own).  A value of g or u that is not
+ *   finite reads back as NaN.
+ *   masked_stride > 0: masked row layout (rows g * stride ..., sizes[g] valid); 0: compact rows.
+ *   tail, tail_cols: NULL, or a [m_rows, tail_cols] 16-bit matrix (another buffer than the operands)
+ *   whose rows behind the last group are set to zero; compact rows only.
+ * Rows of h and saved outside the groups are not written.  Requires k % 8 == 0, inter % 8 == 0,
+ * tail_cols % 8 == 0 and 16-byte aligned base pointers. */
+int b200gemm_m_grouped_gated(const void* a, const void* w13, void* h, void* saved, void* saved_exps, const void* sizes,
+                             int sizes_is_i64, int num_groups, int64_t m_rows, int masked_stride, int inter, int k,
+                             int act, int dtype, void* tail, int tail_cols, int num_sms, void* stream);
+long long b200gemm_gated_exponent_bytes(int64_t m_rows, int inter);
+
+/* dgu [m_rows, 2 inter] = [dh * u * act'(g) | dh * act(g)] with dh = dy w2_e, in one kernel: the gradient
+ * of the gate and up products from the gradient of the block's output.  dy [m_rows, k]; w2 [G, k, inter];
+ * saved, saved_exps: what b200gemm_m_grouped_gated kept for the same rows, sizes, inter and dtype (compact
+ * rows).  tail as above. */
+int b200gemm_m_grouped_gated_grad(const void* dy, const void* w2, const void* saved, const void* saved_exps, void* dgu,
+                                  const void* sizes, int sizes_is_i64, int num_groups, int64_t m_rows, int inter, int k,
+                                  int act, int dtype, void* tail, int tail_cols, int num_sms, void* stream);
+
+/* ---- 4-bit weights with group scales ------------------------------------------------------ */
+
+/* M-grouped product with 4-bit weights, for few rows per expert (decoding):
+ *   c[r, n] = sum_grp scale[g, n, grp] * sum_{k in grp} (q[g, n, k] - zero[g, n, grp]) * a[r, k]
+ * fp32 accumulate, one rounding.  a [m_rows, k] compact rows (bf16 / fp16); w4 [G, N, k/2] bytes, element 2j
+ * in the low and 2j+1 in the high half of byte j; scale [G, N, k/group_size] of a's type; zero
+ * [G, N, k/group_size] bytes (0..15) or NULL (8 everywhere); group_size 32, 64 or 128, k a multiple of it.
+ *   gated == 0: N = n, out [m_rows, n] = c.
+ *   gated != 0: N = 2 n (gate rows, then up rows), out = act(c_gate) * c_up (act as above).
+ * sizes as for b200gemm_m_grouped (cut off at m_rows); at most 1024 groups; n is free of alignment.
+ * Rows of out behind the last group are not written.  Any number of rows per expert is accepted; the kernel
+ * is made for up to a few dozen.  No counterpart in the reference. */
+int b200gemm_w4_m_grouped(const void* a, const void* w4, const void* scale, const void* zero, void* out,
+                          const void* sizes, int sizes_is_i64, int num_groups, int64_t m_rows, int n, int k,
+                          int group_size, int gated, int act, int dtype, int num_sms, void* stream);
+
+/* The quantiser that produces those weights from w [rows, k] 16-bit (finite values), groups of group_size
+ * along k.  zero == NULL: scale = max|w| / 7, q = clamp(round(w / scale) + 8, 0, 15).  Otherwise:
+ * scale = (max(w, 0) - min(w, 0)) / 15, zero = clamp(round(-min / scale), 0, 15),
+ * q = clamp(round(w / scale) + zero, 0, 15).  The scale is rounded to w's type first; rounding is to
+ * nearest even; a group whose rounded scale is 0 holds q = zero = 8 (zero given: 0). */
+int b200quant_w4_group(const void* w, void* q, void* scale, void* zero, int64_t rows, int k, int group_size, int dtype,
+                       void* stream);
+
 /* ---- FP8 grouped GEMMs with per-row x per-channel scales ------------------------------- */
 
 /* FP8 M-grouped GEMM: C[m, n] = (sum_k A[m,k] * B[g,n,k])_fp32 * a_scale[m] * b_scale[g*n_dim+n].
@@ -381,6 +435,26 @@ int b200ipc_close(void* p);
  * copy: contiguous on both sides, so no kernel and no SM is needed for the way back.
  * No counterpart in the reference. */
 int b200ipc_copy_many_async(int n, void* const* dst, const void* const* src, const int64_t* bytes, void* stream);
+
+/* ---- rows between tokens and experts, 16 bits, with gradients (training) -------------------
+ * pos int64 [tokens * top_k] (row of pair p = t * top_k + j) and order int64 [num_rows] (pair of row r)
+ * are the routing plan's two halves.  Pair p owns row r = pos[p] if 0 <= r < num_rows and order[r] == p.
+ * Any other pair - a rejected routing entry's -1, an index given twice - takes no part and raises
+ * B200GEMM_DEV_BAD_ROW_INDEX; a row nobody owns is written as zeros.  top_k <= 32, hidden % 8 == 0, 16-byte
+ * aligned rows.  (Vendored baseline counterparts: grouped_gemm/csrc/permute.cu:40-297 and its backward.) */
+
+/* out[pos[t,j], :] = x[t, :]; x [tokens, hidden], out [num_rows, hidden]. */
+int b200moe_permute_rows(const void* x, const int64_t* pos, const int64_t* order, void* out, int64_t tokens, int top_k,
+                         int hidden, int64_t num_rows, void* stream);
+/* out[t, :] = sum_j weights[t,j] * rows[pos[t,j], :], fp32 accumulate in the order of j, one rounding.
+ * weights == NULL: all ones (the gradient of b200moe_permute_rows). */
+int b200moe_combine_rows(const void* rows, const int64_t* pos, const int64_t* order, const float* weights, void* out,
+                         int64_t tokens, int top_k, int hidden, int64_t num_rows, int dtype, void* stream);
+/* drows[pos[t,j], :] = weights[t,j] * dout[t, :] and dweights[t,j] = <dout[t, :], rows[pos[t,j], :]> (fp32) in one
+ * pass; either may be NULL.  A pair without a row gets dweights = 0. */
+int b200moe_combine_rows_grad(const void* dout, const void* rows, const int64_t* pos, const int64_t* order,
+                              const float* weights, void* drows, float* dweights, int64_t tokens, int top_k, int hidden,
+                              int64_t num_rows, int dtype, void* stream);
 
 /* ---- integer layouts on the device ------------------------------------------------------- */
 

@@ -54,6 +54,18 @@ _SIGNATURES = {
                                             c_int, c_int, c_int, c_int, c_void_p],
     "b200gemm_fp8_k_grouped_block": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int64,
                                      c_int, c_int, c_void_p, c_int64, c_int, c_void_p],
+    "b200gemm_m_grouped_gated": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int64, c_int,
+                                 c_int, c_int, c_int, c_int, c_void_p, c_int, c_int, c_void_p],
+    "b200gemm_m_grouped_gated_grad": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int64,
+                                      c_int, c_int, c_int, c_int, c_void_p, c_int, c_int, c_void_p],
+    "b200gemm_w4_m_grouped": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int64, c_int,
+                              c_int, c_int, c_int, c_int, c_int, c_int, c_void_p],
+    "b200quant_w4_group": [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_void_p],
+    "b200moe_permute_rows": [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_int64, c_void_p],
+    "b200moe_combine_rows": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_int64, c_int,
+                             c_void_p],
+    "b200moe_combine_rows_grad": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int,
+                                  c_int, c_int64, c_int, c_void_p],
     "b200moe_route_plan": [c_void_p, c_int64, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
     "b200moe_route_plan_mapped": [c_void_p, c_int64, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
     "b200moe_peer_plan": [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_int64, c_int, c_void_p,
@@ -86,7 +98,8 @@ _SIGNATURES = {
                                     c_int64, c_int, c_void_p],
 }
 
-EXPORTED_SYMBOLS = tuple(_SIGNATURES) + ("b200gemm_last_error", "b200gemm_k_grouped_workspace_bytes")
+EXPORTED_SYMBOLS = tuple(_SIGNATURES) + ("b200gemm_last_error", "b200gemm_k_grouped_workspace_bytes",
+                                           "b200gemm_gated_exponent_bytes")
 
 
 def load():
@@ -113,6 +126,8 @@ def load():
         lib.b200gemm_last_error.restype = c_char_p
         lib.b200gemm_k_grouped_workspace_bytes.argtypes = [c_int]
         lib.b200gemm_k_grouped_workspace_bytes.restype = ctypes.c_longlong
+        lib.b200gemm_gated_exponent_bytes.argtypes = [c_int64, c_int]
+        lib.b200gemm_gated_exponent_bytes.restype = ctypes.c_longlong
         _lib = lib
     return _lib
 
@@ -141,6 +156,12 @@ def stream_ptr(device: torch.device) -> int:
 
 def ptr(t: torch.Tensor) -> int:
     return t.data_ptr()
+
+
+def aligned(t: torch.Tensor) -> torch.Tensor:
+    """``t``, or a copy of it if it is not contiguous or not 16-byte aligned (a gradient that autograd hands over)."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 def device_status(clear: bool = True) -> int:

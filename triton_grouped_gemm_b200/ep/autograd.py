@@ -1,0 +1,129 @@
+"""Differentiable row movement between tokens and experts on one rank, and the trainable MoE layer made of it.
+
+``pos`` (row of pair p = t * top_k + j) and ``order`` (pair of row r) are the two halves of a routing plan:
+``make_plan(topk_idx, num_experts)`` gives them as ``plan.pos`` and ``plan.send_order``.  A pair whose ``pos`` is
+out of range (the -1 of a dropped token) or whose row's ``order`` names another pair takes no part and raises
+status bit ``0x20``; a row that no pair owns reads as zeros.  The forward-only movers of the FP8 layer are in
+``ep.dispatch``; the reference has these operators only in its vendored baseline (grouped_gemm/ops.py permute /
+unpermute).
+"""
+
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .. import _lib
+from ..gemm.autograd import grouped_gated_ffn
+from .dispatch import make_plan
+
+
+def _check_plan(what: str, pos: torch.Tensor, order: torch.Tensor, pairs: int, device) -> None:
+    assert pos.dtype == torch.int64 and order.dtype == torch.int64, f"{what}: pos and order must be int64"
+    assert pos.numel() == pairs and pos.is_contiguous() and order.is_contiguous() and order.dim() == 1, \
+        f"{what}: pos must hold one contiguous entry per (token, k) pair and order one per row"
+    _lib.require_cuda(pos, order)
+    assert pos.device == device and order.device == device, f"{what}: all operands must be on one device"
+
+
+def _permute(x, pos, order, top_k):
+    t, h = x.shape
+    out = x.new_empty(order.numel(), h)
+    with torch.cuda.device(x.device):
+        rc = _lib.load().b200moe_permute_rows(x.data_ptr(), pos.data_ptr(), order.data_ptr(), out.data_ptr(), t, top_k, h,
+                                              order.numel(), _lib.stream_ptr(x.device))
+    _lib.check(rc, "b200moe_permute_rows")
+    return out
+
+
+def _combine(rows, w32, pos, order, tokens, top_k):
+    r, h = rows.shape
+    out = rows.new_empty(tokens, h)
+    with torch.cuda.device(rows.device):
+        rc = _lib.load().b200moe_combine_rows(rows.data_ptr(), pos.data_ptr(), order.data_ptr(),
+                                              w32.data_ptr() if w32 is not None else None, out.data_ptr(), tokens, top_k, h, r,
+                                              _lib.dtype_code(rows.dtype), _lib.stream_ptr(rows.device))
+    _lib.check(rc, "b200moe_combine_rows")
+    return out
+
+
+class _PermuteRows(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, pos, order, top_k):
+        ctx.save_for_backward(pos, order)
+        ctx.top_k = top_k
+        return _permute(x, pos, order, top_k)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, drows):
+        pos, order = ctx.saved_tensors
+        return _combine(_lib.aligned(drows), None, pos, order, pos.numel() // ctx.top_k, ctx.top_k), None, None, None
+
+
+class _CombineRows(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, rows, topk_weight, pos, order):
+        t, top_k = topk_weight.shape
+        w32 = topk_weight.to(torch.float32).contiguous()
+        ctx.save_for_backward(rows if ctx.needs_input_grad[1] else None, w32, pos, order)
+        ctx.num_rows, ctx.weight_dtype = rows.shape[0], topk_weight.dtype
+        return _combine(rows, w32, pos, order, t, top_k)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        rows, w32, pos, order = ctx.saved_tensors
+        dout = _lib.aligned(dout)
+        t, h = dout.shape
+        drows = dout.new_empty(ctx.num_rows, h) if ctx.needs_input_grad[0] else None
+        dw = torch.empty_like(w32) if ctx.needs_input_grad[1] else None
+        with torch.cuda.device(dout.device):
+            rc = _lib.load().b200moe_combine_rows_grad(
+                dout.data_ptr(), rows.data_ptr() if rows is not None else None, pos.data_ptr(), order.data_ptr(),
+                w32.data_ptr(), drows.data_ptr() if drows is not None else None, dw.data_ptr() if dw is not None else None,
+                t, w32.shape[1], h, ctx.num_rows, _lib.dtype_code(dout.dtype), _lib.stream_ptr(dout.device))
+        _lib.check(rc, "b200moe_combine_rows_grad")
+        return drows, dw.to(ctx.weight_dtype) if dw is not None else None, None, None
+
+
+def permute_rows(x: torch.Tensor, pos: torch.Tensor, order: torch.Tensor, top_k: int) -> torch.Tensor:
+    """x [T, H] bf16 / fp16 -> rows [R, H] with ``rows[pos[t * top_k + j]] = x[t]`` (R = order.numel()), differentiable
+    in x.  H a multiple of 8, top_k <= 32."""
+    assert x.dim() == 2, "x must be 2D [T, H]"
+    _lib.dtype_code(x.dtype)
+    _lib.require_cuda(x)
+    _check_plan("permute_rows", pos, order, x.shape[0] * top_k, x.device)
+    x = x.contiguous()
+    if torch.is_grad_enabled() and x.requires_grad:
+        return _PermuteRows.apply(x, pos, order, top_k)
+    return _permute(x, pos, order, top_k)
+
+
+def combine_rows(rows: torch.Tensor, topk_weight: torch.Tensor, pos: torch.Tensor, order: torch.Tensor) -> torch.Tensor:
+    """rows [R, H] bf16 / fp16, topk_weight [T, k] -> [T, H] with ``out[t] = sum_j topk_weight[t, j] *
+    rows[pos[t * k + j]]`` (fp32 sums), differentiable in rows and topk_weight.  H a multiple of 8, k <= 32."""
+    assert rows.dim() == 2 and topk_weight.dim() == 2, "rows must be 2D [R, H] and topk_weight 2D [T, k]"
+    assert topk_weight.is_floating_point(), "topk_weight must be floating point"
+    assert order.numel() == rows.shape[0], "order must have one entry per row"
+    _lib.dtype_code(rows.dtype)
+    _lib.require_cuda(rows, topk_weight)
+    assert topk_weight.device == rows.device, "combine_rows: all operands must be on one device"
+    _check_plan("combine_rows", pos, order, topk_weight.numel(), rows.device)
+    rows = rows.contiguous()
+    if torch.is_grad_enabled() and (rows.requires_grad or topk_weight.requires_grad):
+        return _CombineRows.apply(rows, topk_weight, pos, order)
+    t, top_k = topk_weight.shape
+    return _combine(rows, topk_weight.to(torch.float32).contiguous(), pos, order, t, top_k)
+
+
+def moe_ffn(x: torch.Tensor, topk_idx: torch.Tensor, topk_weight: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor,
+            activation: str = "silu") -> torch.Tensor:
+    """Trainable 16-bit MoE feed-forward layer on one rank: x [T, H], topk_idx [T, k] (an id outside the experts drops
+    the pair), topk_weight [T, k], w13 [E, 2*I, H] (gate rows, then up rows), w2 [E, H, I] -> [T, H], with gradients
+    for x, topk_weight, w13 and w2.  Nothing synchronises the host."""
+    top_k = topk_idx.shape[1]
+    plan = make_plan(topk_idx, w13.shape[0])
+    rows = permute_rows(x, plan.pos, plan.send_order, top_k)
+    y = grouped_gated_ffn(rows, w13, w2, plan.size_per_group, activation)
+    return combine_rows(y, topk_weight, plan.pos, plan.send_order)

@@ -1,5 +1,6 @@
 """Differentiable grouped GEMM: forward and input gradient through the M-grouped kernel, weight
-gradient through the K-grouped kernel (16-bit, and block-scaled FP8 throughout in ``grouped_gemm_fp8``).
+gradient through the K-grouped kernel (16-bit, and block-scaled FP8 throughout in ``grouped_gemm_fp8``);
+and the experts' gated feed-forward block, ``grouped_gated_ffn``.
 
 The reference keeps forward (``m_grouped_gemm``) and weight gradient (``k_grouped_gemm``) as
 separate operators; its vendored baseline wraps the cuBLAS loop in an autograd function
@@ -14,8 +15,11 @@ separate operators; its vendored baseline wraps the cuBLAS loop in an autograd f
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
+from .. import _lib
 from .BF16.k_grouped_gemm_TMA import k_grouped_gemm
+from .BF16.m_grouped_gated_gemm import _m_grouped_gated_grad_launch, _m_grouped_gated_launch
 from .BF16.m_grouped_gemm_TMA import _m_grouped_gemm_launch
 
 
@@ -101,3 +105,64 @@ def grouped_gemm_fp8(a: torch.Tensor, b: torch.Tensor, size_per_group: torch.Ten
     weight gradient (16-bit when ``fp8_wgrad`` is False or K / N are not multiples of 128).
     ``a`` [M, K] and ``b`` [G, N, K] are bf16."""
     return _GroupedGemmFp8.apply(a, b, size_per_group, fp8_wgrad)
+
+
+class _GroupedGatedFfn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w13, w2, size_per_group, activation):
+        need_x, need_w13, need_w2 = ctx.needs_input_grad[:3]
+        h, saved, exps, y = _gated_ffn_forward(x, w13, w2, size_per_group, activation, save=need_x or need_w13)
+        ctx.save_for_backward(x if need_w13 else None, w13 if need_x else None, w2 if need_x or need_w13 else None,
+                              h if need_w2 else None, saved, exps, size_per_group)
+        ctx.activation = activation
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, w13, w2, h, saved, exps, size_per_group = ctx.saved_tensors
+        need_x, need_w13, need_w2 = ctx.needs_input_grad[:3]
+        dy = _lib.aligned(dy)
+        dx = dw13 = dw2 = None
+        if need_x or need_w13:
+            if need_x:
+                dx = dy.new_empty(dy.shape)   # [M, H]: zeroed behind the last group, then filled below
+            dgu = _m_grouped_gated_grad_launch(dy, w2, saved, exps, size_per_group, ctx.activation, tail=dx)
+            if need_x:
+                _m_grouped_gemm_launch(dgu, w13, dx, size_per_group, False)
+            if need_w13:
+                dw13 = k_grouped_gemm(dgu, x, size_per_group)
+        if need_w2:
+            dw2 = k_grouped_gemm(dy, h, size_per_group)
+        return dx, dw13, dw2, None, None
+
+
+def _gated_ffn_forward(x, w13, w2, size_per_group, activation, save):
+    y = x.new_empty(x.shape)
+    h, saved, exps = _m_grouped_gated_launch(x, w13, size_per_group, activation, save=save, tail=y)
+    _m_grouped_gemm_launch(h, w2, y, size_per_group, True)
+    return h, saved, exps, y
+
+
+def grouped_gated_ffn(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, size_per_group: torch.Tensor,
+                      activation: str = "silu"):
+    """The experts' gated feed-forward block ``y = (act(x @ Wg_g.T) * (x @ Wu_g.T)) @ W2_g.T`` with gradients for
+    x, w13 and w2.  x [M, H] rows grouped by expert, w13 [G, 2*I, H] (gate rows, then up rows), w2 [G, H, I], all
+    bf16 or all fp16, H and I multiples of 8; ``activation`` "silu" or "gelu_tanh".  Rows behind
+    ``sum(size_per_group)`` give zero rows of y and of x's gradient.
+
+    Two kernels forward (gate+up product with the gate in its epilogue, down product) and four backward (the down
+    product's gradient with the gate's derivative in its epilogue, dx, dW13, dW2).  For the gradients the block
+    keeps x, h [M, I] and the gate and up products in 16-bit block floating point."""
+    assert x.dim() == 2 and w2.dim() == 3, "x must be 2D [M, H] and w2 3D [num_groups, H, I]"
+    assert tuple(w2.shape) == (w13.shape[0], x.shape[1], w13.shape[1] // 2), "w2 should have shape [num_groups, H, I]"
+    assert x.shape[1] > 0 and w2.shape[2] > 0, "H and I must be positive"
+    assert w2.dtype == x.dtype, "x, w13 and w2 must share one dtype"
+    _lib.require_cuda(x, w13, w2, size_per_group)
+    assert x.device == w2.device, "x, w13, w2 and size_per_group must be on one device"
+    x, w13, w2 = x.contiguous(), w13.contiguous(), w2.contiguous()
+    if size_per_group.dtype not in (torch.int32, torch.int64):
+        size_per_group = size_per_group.to(torch.int64)
+    if torch.is_grad_enabled() and (x.requires_grad or w13.requires_grad or w2.requires_grad):
+        return _GroupedGatedFfn.apply(x, w13, w2, size_per_group, activation)
+    return _gated_ffn_forward(x, w13, w2, size_per_group, activation, save=False)[3]
