@@ -10,8 +10,10 @@ import torch
 
 HALF_EPS = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
 HALF_TINY = {torch.bfloat16: 2.0 ** -134, torch.float16: 2.0 ** -25}
-# block floating point of the kept gate and up values: half a mantissa step, half a denormal step of the block maximum
-KEPT = {torch.bfloat16: (2.0 ** -12, 2.0 ** -25), torch.float16: (2.0 ** -13, 2.0 ** -18)}
+# the kept gate and up values, relative to themselves and to their block's maximum: half a mantissa step and half a
+# denormal step.  bf16 layers: fp16 with the maximum in [2^14, 2^15): 2^-11 and 2^-25 / 2^14.  fp16 layers: 12 mantissa
+# bits, 2^-13, down to 2^-5 of the maximum's power of two, in steps of 2^-17 of it below: 2^-18.
+KEPT = {torch.bfloat16: (2.0 ** -11, 2.0 ** -39), torch.float16: (2.0 ** -13, 2.0 ** -18)}
 
 
 def act_and_slopes(g, act):

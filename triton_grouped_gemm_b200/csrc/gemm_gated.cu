@@ -23,6 +23,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "../../include/b200gemm.h"
 #include "activation.cuh"
 #include "common.cuh"
@@ -33,50 +35,75 @@ namespace b200 {
 enum class GatedMode { kForward, kForwardSave, kBackward };
 
 // ------------------------------------------------------------------ block floating point
-// A block of 32 values is scaled by a power of two so that the largest has the fp32 exponent field kTop, rounded
-// to kMant mantissa bits, and the (then zero) upper exponent bits are dropped: 1 sign, 15 - kMant exponent and kMant
-// mantissa bits.  Values far below the block's maximum become denormal in that scale, in even steps of 2^-kMant of
-// its smallest normal value.  The all-ones code stands for a value that was not finite and reads back as NaN.
-template <bool kFp16>
-struct BlockFloat {
-  static constexpr int kMant = kFp16 ? 12 : 11;
-  static constexpr int kDrop = 23 - kMant;
-  static constexpr int kTop = (1 << (15 - kMant)) - 2;  // one below all ones: rounding may carry into the exponent
-};
+// A block of 32 values v is kept as 16-bit codes and the fp32 exponent field e of its largest finite magnitude.
+//   bf16 layers   code = fp16(v * 2^(141 - e)): the largest lies in [2^14, 2^15), 10 mantissa bits down to 2^-28 of it.
+//                 One multiplication and half a conversion per value, and fp16's own infinities and NaN.
+//   fp16 layers   fp16 would add as much error as the output's rounding, so one exponent bit more is given to the
+//                 mantissa twice over: v is scaled until the largest has exponent field kTop, rounded to 12 bits in
+//                 integer arithmetic, and the 5 upper exponent bits, then zero, are dropped: 1 sign, 3 exponent, 12
+//                 mantissa bits, even steps of 2^-17 of the largest's power of two below 2^-5 of it.  The all-ones
+//                 code stands for a value that was not finite and reads back as NaN.
+constexpr uint32_t kBlockExpMin = 15;   // keeps 2^(141 - e) and its inverse normal numbers
+constexpr int kCodeMant = 12;
+constexpr int kCodeDrop = 23 - kCodeMant;
+constexpr uint32_t kCodeTop = 6;        // one below all ones (7): rounding may carry into the exponent
 
-// the exponent field (1..254) of the largest finite magnitude
 __device__ __forceinline__ uint32_t block_exponent(const uint32_t (&v)[32]) {
-  uint32_t m = 0;
+  float m = 0.f;
 #pragma unroll
-  for (int i = 0; i < 32; ++i) {
-    const uint32_t a = v[i] & 0x7FFFFFFFu;
-    m = max(m, a < 0x7F800000u ? a : 0u);
+  for (int i = 0; i < 32; ++i) m = fmaxf(m, fabsf(__uint_as_float(v[i])));   // NaN is passed over
+  if (m > 3.0e38f) {                                                         // rare: look again, without infinities
+    m = 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const float a = fabsf(__uint_as_float(v[i]));
+      if (a < __uint_as_float(0x7F800000u)) m = fmaxf(m, a);
+    }
   }
-  return max(m >> 23, 1u);
+  return max(__float_as_uint(m) >> 23, kBlockExpMin);
 }
 
-// 2^(127 - e) for an exponent field e of 1..254 (e = 254: the denormal 2^-127)
-__device__ __forceinline__ float block_down(uint32_t e) {
-  return __uint_as_float(e < 254u ? (254u - e) << 23 : 0x00400000u);
-}
-
+// 2^(141 - e), e in [15, 254]
+__device__ __forceinline__ float block_down(uint32_t e) { return __uint_as_float((268u - e) << 23); }
+// bf16 layers: its inverse; fp16 layers: 2^(e - 127), what is left after the code's own 2^121
 template <bool kFp16>
-__device__ __forceinline__ uint32_t encode1(uint32_t v, float down) {
-  using F = BlockFloat<kFp16>;
-  const float to_field = __uint_as_float(static_cast<uint32_t>(F::kTop) << 23);  // 2^(kTop - 127): [1, 2) -> field kTop
-  const uint32_t f = __float_as_uint(__uint_as_float(v) * down * to_field);
+__device__ __forceinline__ float block_up(uint32_t e) {
+  return __uint_as_float((kFp16 ? e : e - 14u) << 23);
+}
+
+__device__ __forceinline__ uint32_t code12(uint32_t v, float down) {
+  // times 2^-135 (a denormal): [2^14, 2^15) -> [2^-121, 2^-120), whose exponent field is kCodeTop
+  const uint32_t f = __float_as_uint(__uint_as_float(v) * down * __uint_as_float(1u << 14));
   const uint32_t mag = f & 0x7FFFFFFFu;
-  const uint32_t code = (mag + ((1u << (F::kDrop - 1)) - 1) + ((mag >> F::kDrop) & 1u)) >> F::kDrop;
+  const uint32_t code = (mag + ((1u << (kCodeDrop - 1)) - 1) + ((mag >> kCodeDrop) & 1u)) >> kCodeDrop;
   return min(code, 0x7FFFu) | ((f >> 16) & 0x8000u);
 }
 
 template <bool kFp16>
-__device__ __forceinline__ float decode1(uint32_t code, float up) {
-  using F = BlockFloat<kFp16>;
-  const float from_field = __uint_as_float(static_cast<uint32_t>(254 - F::kTop) << 23);  // 2^(127 - kTop)
-  const uint32_t mag = code & 0x7FFFu;
-  const float f = __uint_as_float((mag << F::kDrop) | ((code & 0x8000u) << 16)) * from_field * up;
-  return mag == 0x7FFFu ? __uint_as_float(0x7FFFFFFFu) : f;
+__device__ __forceinline__ uint32_t encode2(uint32_t lo, uint32_t hi, float down) {
+  if constexpr (!kFp16) return pack2_16bit(__uint_as_float(lo) * down, __uint_as_float(hi) * down, 1);
+  return code12(lo, down) | code12(hi, down) << 16;
+}
+
+template <bool kFp16>
+__device__ __forceinline__ float2 decode2(uint32_t codes, float up) {
+  if constexpr (!kFp16) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&codes));
+    return make_float2(f.x * up, f.y * up);
+  }
+  auto one = [&](uint32_t code) {
+    const uint32_t mag = code & 0x7FFFu;
+    const float f = __uint_as_float((mag << kCodeDrop) | ((code & 0x8000u) << 16)) * __uint_as_float((127u + 127u - kCodeTop) << 23) * up;
+    return mag == 0x7FFFu ? __uint_as_float(0x7FFFFFFFu) : f;
+  };
+  return make_float2(one(codes & 0xFFFFu), one(codes >> 16));
+}
+
+// runs f with the activation as a compile-time constant
+template <typename F>
+__device__ __forceinline__ void with_activation(int act, F&& f) {
+  if (act == kActSilu) f(std::integral_constant<int, kActSilu>{});
+  else f(std::integral_constant<int, kActGeluTanh>{});
 }
 
 // ------------------------------------------------------------------ kernel
@@ -134,7 +161,7 @@ gated_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ C
   constexpr int kTileRows = kPair ? 256 : 128;
   constexpr int kCtaGroup = kPair ? 2 : 1;
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);   // still known to be shared memory
   const uint32_t smem_base = smem_u32(smem);
   const uint32_t bar_base = smem_base + L::kBarOffset;
   auto full_bar = [&](int s) { return bar_base + 8u * s; };
@@ -375,17 +402,20 @@ gated_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ C
                 if (full) *reinterpret_cast<uint4*>(buf + row_off + ((static_cast<uint32_t>(s * 4 + v) ^ swz) << 4)) = vec;
                 else if (row_ok && col0 + s * 32 + v * 8 < p.inter) *reinterpret_cast<uint4*>(global + s * 32 + v * 8) = vec;
               };
+              with_activation(p.act, [&](auto act) {
+                constexpr int kAct = decltype(act)::value;
 #pragma unroll
               for (int v = 0; v < 4; ++v) {
                 uint32_t q[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                   const int i = v * 8 + e * 2;
-                  q[e] = pack2_16bit(gate_value(__uint_as_float(g[i]), p.act) * __uint_as_float(u[i]),
-                                     gate_value(__uint_as_float(g[i + 1]), p.act) * __uint_as_float(u[i + 1]), kFp16);
+                  q[e] = pack2_16bit(gate_value<kAct>(__uint_as_float(g[i])) * __uint_as_float(u[i]),
+                                     gate_value<kAct>(__uint_as_float(g[i + 1])) * __uint_as_float(u[i + 1]), kFp16);
                 }
                 put(buf_h, p.h + row * p.inter + col0, v, q);
               }
+              });
               if constexpr (kSave) {
                 const uint32_t eg = block_exponent(g), eu = block_exponent(u);
                 const float down_g = block_down(eg), down_u = block_down(eu);
@@ -398,8 +428,8 @@ gated_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ C
 #pragma unroll
                   for (int e = 0; e < 4; ++e) {
                     const int i = v * 8 + e * 2;
-                    qg[e] = encode1<kFp16>(g[i], down_g) | encode1<kFp16>(g[i + 1], down_g) << 16;
-                    qu[e] = encode1<kFp16>(u[i], down_u) | encode1<kFp16>(u[i + 1], down_u) << 16;
+                    qg[e] = encode2<kFp16>(g[i], g[i + 1], down_g);
+                    qu[e] = encode2<kFp16>(u[i], u[i + 1], down_u);
                   }
                   put(buf_g, gu_row, v, qg);
                   put(buf_u, gu_row + p.inter, v, qu);
@@ -456,9 +486,11 @@ gated_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ C
               uint32_t dh[32];
               tmem_ld_32x32b_x32(t_addr + c * 64 + s * 32, dh);
               const int shift = 8 * ((c & 1) * 2 + s);
-              const float up_g = __uint_as_float(((word_g >> shift) & 0xFFu) << 23);
-              const float up_u = __uint_as_float(((word_u >> shift) & 0xFFu) << 23);
+              const float up_g = block_up<kFp16>((word_g >> shift) & 0xFFu);
+              const float up_u = block_up<kFp16>((word_u >> shift) & 0xFFu);
               tmem_ld_wait();
+              with_activation(p.act, [&](auto act) {
+              constexpr int kAct = decltype(act)::value;
 #pragma unroll
               for (int v = 0; v < 4; ++v) {
                 uint4* at_g = reinterpret_cast<uint4*>(buf + row_off + ((static_cast<uint32_t>(s * 4 + v) ^ swz) << 4));
@@ -468,19 +500,13 @@ gated_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ C
                 uint32_t qg[4], qu[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                  float dg[2], du[2];
-#pragma unroll
-                  for (int b = 0; b < 2; ++b) {
-                    const float g = decode1<kFp16>((wg[e] >> (16 * b)) & 0xFFFFu, up_g);
-                    const float u = decode1<kFp16>((wu[e] >> (16 * b)) & 0xFFFFu, up_u);
-                    const float d = __uint_as_float(dh[v * 8 + e * 2 + b]);
-                    float value, slope;
-                    gate_value_slope(g, p.act, value, slope);
-                    dg[b] = d * u * slope;
-                    du[b] = d * value;
-                  }
-                  qg[e] = pack2_16bit(dg[0], dg[1], kFp16);
-                  qu[e] = pack2_16bit(du[0], du[1], kFp16);
+                  const float2 g = decode2<kFp16>(wg[e], up_g), u = decode2<kFp16>(wu[e], up_u);
+                  const float d0 = __uint_as_float(dh[v * 8 + e * 2]), d1 = __uint_as_float(dh[v * 8 + e * 2 + 1]);
+                  float value0, value1, slope0, slope1;
+                  gate_value_slope<kAct>(g.x, value0, slope0);
+                  gate_value_slope<kAct>(g.y, value1, slope1);
+                  qg[e] = pack2_16bit(d0 * u.x * slope0, d1 * u.y * slope1, kFp16);
+                  qu[e] = pack2_16bit(d0 * value0, d1 * value1, kFp16);
                 }
                 const uint4 og = make_uint4(qg[0], qg[1], qg[2], qg[3]), ou = make_uint4(qu[0], qu[1], qu[2], qu[3]);
                 if (full) {
@@ -492,6 +518,7 @@ gated_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ C
                   *reinterpret_cast<uint4*>(d + p.inter) = ou;
                 }
               }
+              });
               // the next chunk's codes travel while the second half of this one is worked on
               if (s == 0 && c + 1 < kCols / 64 && col0 + 64 < p.inter) ask(c + 1);
             }

@@ -133,8 +133,9 @@ permute_rows_kernel(const uint4* __restrict__ x, const long long* __restrict__ p
 }
 
 // out[t] = sum_j w[t,j] * rows[pos[t,j]] in the order of j; weights == nullptr: all ones (the gradient of permute).
-// kK rows' loads of a vector are issued together; top_k > kK takes further rounds.
-template <bool kSpread, int kK, bool kFp16>
+// kK rows' loads of kU vectors are issued together; top_k > kK takes further rounds (kRounds), with the rows' addresses
+// fetched anew from the lanes that hold them.
+template <bool kSpread, int kK, int kU, bool kRounds, bool kFp16>
 __global__ void __launch_bounds__(kRowsThreads)
 combine_rows_kernel(const uint4* __restrict__ rows, const long long* __restrict__ pos,
                     const long long* __restrict__ order, const float* __restrict__ weights, uint4* __restrict__ out,
@@ -144,32 +145,46 @@ combine_rows_kernel(const uint4* __restrict__ rows, const long long* __restrict_
   for (long long t = w.first; t < tokens; t += w.stride) {
     const long long mine = owned_row(pos, order, t, top_k, num_rows, w.lane, status);
     const float my_weight = w.lane < top_k ? (weights ? weights[t * top_k + w.lane] : 1.f) : 0.f;
-    for (int vb = w.vb0; vb < row_vecs; vb += kStep) {
-      const int v = vb + w.lane;
-      float acc[8];
+    const uint4* src[kK];   // nullptr: no row
+    float wk[kK];
+    auto fetch = [&](int j0) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) acc[e] = 0.f;
-      for (int j0 = 0; j0 < top_k; j0 += kK) {
-        uint4 q[kK];
-        float wk[kK];
-        bool use[kK];
-#pragma unroll
-        for (int j = 0; j < kK; ++j) {
-          const long long r = __shfl_sync(0xFFFFFFFFu, mine, (j0 + j) & 31);
-          wk[j] = __shfl_sync(0xFFFFFFFFu, my_weight, (j0 + j) & 31);
-          use[j] = j0 + j < top_k && r >= 0 && v < row_vecs;
-          if (use[j]) q[j] = __ldg(rows + r * row_vecs + v);
-        }
-#pragma unroll
-        for (int j = 0; j < kK; ++j) {
-          if (!use[j]) continue;
-          float f[8];
-          unpack8<kFp16>(q[j], f);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) acc[e] = fmaf(wk[j], f[e], acc[e]);
-        }
+      for (int j = 0; j < kK; ++j) {
+        const long long r = __shfl_sync(0xFFFFFFFFu, mine, (j0 + j) & 31);
+        wk[j] = __shfl_sync(0xFFFFFFFFu, my_weight, (j0 + j) & 31);
+        src[j] = j0 + j < top_k && r >= 0 ? rows + r * row_vecs : nullptr;
       }
-      if (v < row_vecs) out[t * row_vecs + v] = pack8<kFp16>(acc);
+    };
+    if constexpr (!kRounds) fetch(0);
+    for (int vb = w.vb0; vb < row_vecs; vb += kU * kStep) {
+      const int v = vb + w.lane;
+      float acc[kU][8];
+#pragma unroll
+      for (int i = 0; i < kU; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[i][e] = 0.f;
+      for (int j0 = 0; j0 < (kRounds ? top_k : 1); j0 += kK) {
+        if constexpr (kRounds) fetch(j0);
+        uint4 q[kU][kK];
+#pragma unroll
+        for (int i = 0; i < kU; ++i)
+#pragma unroll
+          for (int j = 0; j < kK; ++j)
+            if (src[j] && v + i * kStep < row_vecs) q[i][j] = __ldg(src[j] + v + i * kStep);
+#pragma unroll
+        for (int i = 0; i < kU; ++i)
+#pragma unroll
+          for (int j = 0; j < kK; ++j) {
+            if (!src[j]) continue;
+            float f[8];
+            unpack8<kFp16>(q[i][j], f);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[i][e] = fmaf(wk[j], f[e], acc[i][e]);
+          }
+      }
+#pragma unroll
+      for (int i = 0; i < kU; ++i)
+        if (v + i * kStep < row_vecs) out[t * row_vecs + v + i * kStep] = pack8<kFp16>(acc[i]);
     }
   }
 }
@@ -316,10 +331,11 @@ template <bool kSpread, bool kFp16>
 static void launch_combine(int top_k, unsigned grid, cudaStream_t stream, const uint4* rows, const long long* pos,
                            const long long* order, const float* weights, uint4* out, long long tokens, int row_vecs,
                            long long num_rows) {
-  auto kern = top_k == 1   ? combine_rows_kernel<kSpread, 1, kFp16>
-              : top_k == 2 ? combine_rows_kernel<kSpread, 2, kFp16>
-              : top_k <= 4 ? combine_rows_kernel<kSpread, 4, kFp16>
-                           : combine_rows_kernel<kSpread, 8, kFp16>;
+  auto kern = top_k == 1   ? combine_rows_kernel<kSpread, 1, 4, false, kFp16>
+              : top_k == 2 ? combine_rows_kernel<kSpread, 2, 4, false, kFp16>
+              : top_k <= 4 ? combine_rows_kernel<kSpread, 4, 2, false, kFp16>
+              : top_k <= 8 ? combine_rows_kernel<kSpread, 8, 1, false, kFp16>
+                           : combine_rows_kernel<kSpread, 8, 1, true, kFp16>;
   kern<<<grid, kRowsThreads, 0, stream>>>(rows, pos, order, weights, out, tokens, top_k, row_vecs, num_rows,
                                           device_status_ptr());
 }

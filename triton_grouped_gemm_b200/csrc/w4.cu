@@ -17,12 +17,17 @@
 //     per 8 values) and the weights stay in their natural order in memory.
 //
 // A block takes a tile of kWN * 32 weight rows of one expert (gated: half gate, half up rows) and up to kNT * 8 rows
-// of `a`.  kWK warps split each 256-wide stage of k; their partial sums are joined in shared memory in a fixed order,
-// so results do not depend on timing.  Stages are fetched with 16-byte cp.async, kStages of them in flight.  Blocks
-// are persistent over the (expert with rows, row chunk, tile) items; an expert's row chunks are neighbours, so the
-// second one finds the weights in L2.
+// of `a`.  kWK warps split each stage of kSB * 32 k; their partial sums are joined in a fixed order, so results do not
+// depend on timing.  Blocks are persistent over the (expert with rows, tile, row chunk) items; an expert's row chunks
+// are neighbours, so the second one finds the weights in L2.  Of two further warps one fetches the stages by TMA and
+// one the scales, both running ahead across the items' borders, so a block never drains, and the multiplying warps
+// meet only to join their sums.  The 128-byte swizzle makes both operands' fragment loads free of bank conflicts (rows of `a` are taken in
+// the order 0 4 1 5 2 6 3 7 for that).  With the loads off the warps' hands the kernel is bound by the logic
+// pipe (masks, shifts, byte permutes: 24 instructions per 32 x 32 values in fp16, 32 in bf16) until HBM takes over.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <type_traits>
 
 #include "../../include/b200gemm.h"
 #include "activation.cuh"
@@ -30,16 +35,10 @@
 
 namespace b200 {
 
-constexpr int kW4Threads = 256;
-constexpr int kW4StageK = 256;        // k per stage: 128 bytes of a weight row
-constexpr int kW4RowBytes = 128 + 16; // stage pitch of a weight row: an odd number of 16-byte units, conflict-free
-constexpr int kW4ABytes = 512 + 64;   // stage pitch of a row of `a`: 64 modulo 128, conflict-free 16-byte loads
-constexpr int kW4WindowGroups = 128;  // scales are staged for this many groups at a time
+constexpr int kW4WindowGroups = 32;   // scales are staged for this many groups at a time
 constexpr int kW4MaxGroups = 1024;    // experts
 
 struct W4Args {
-  const uint8_t* a;      // [m_rows, k] 16-bit
-  const uint8_t* w;      // [G, weight rows, k / 2]
   const uint8_t* scale;  // [G, weight rows, k / group_size] 16-bit
   const uint8_t* zero;   // same, bytes, or null (zero = 8)
   uint16_t* out;         // [m_rows, n]
@@ -48,11 +47,12 @@ struct W4Args {
   int num_groups;
   long long m_rows;
   int n, k;
-  int log_gs32;          // log2(group_size / 32)
   int act;
   int tiles;             // tiles per expert
-  int scale_pitch;       // bytes per row of the staged scales / zeros
+  int scale_pitch;       // bytes per row of the staged scales / zeros: odd numbers of 16-byte units, conflict-free
   int zero_pitch;
+  int log_scale_vecs;    // log2 of the 16-byte pieces (rounded up to a power of two) of a row's staged scales / zeros
+  int log_zero_vecs;
   int list_capacity;     // entries of the list of experts with rows
   unsigned* status;
 };
@@ -64,32 +64,7 @@ struct W4Expert {
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
-__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
-  uint32_t v;
-  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr));
-  return v;
-}
-__device__ __forceinline__ uint32_t lds16(uint32_t addr) {
-  uint16_t v;
-  asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(addr));
-  return v;
-}
-__device__ __forceinline__ uint32_t lds8(uint32_t addr) {
-  uint32_t v;
-  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(addr));
-  return v;
-}
-__device__ __forceinline__ uint4 lds128(uint32_t addr) {
-  uint4 v;
-  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
-  return v;
-}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 template <bool kFp16>
 __device__ __forceinline__ float to_float(uint32_t bits) {
@@ -97,18 +72,25 @@ __device__ __forceinline__ float to_float(uint32_t bits) {
   return __uint_as_float(bits << 16);
 }
 
-// d = a * b + d, a: 16 weight rows x 16 k, b: 16 k x 8 rows of the activations
-template <bool kFp16>
+// d = a * b + c, a: 16 weight rows x 16 k, b: 16 k x 8 rows of the activations; kFirst: c = 0
+template <bool kFp16, bool kFirst>
 __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  const float c0 = kFirst ? 0.f : d[0], c1 = kFirst ? 0.f : d[1], c2 = kFirst ? 0.f : d[2], c3 = kFirst ? 0.f : d[3];
   if constexpr (kFp16)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
   else
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+}
+
+// (w & mask) | magic in one instruction
+__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t magic) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(w), "r"(mask), "r"(magic));
+  return r;
 }
 
 template <bool kFp16>
@@ -128,57 +110,106 @@ __device__ __forceinline__ uint32_t zero_pair(uint32_t zero) {
   return ((kFp16 ? 0x6400u : 0x4300u) + zero) * 0x10001u;
 }
 
-// the four pairs (0,4) (1,5) (2,6) (3,7) of a word of eight 4-bit values, minus their zero
+// the four pairs (0,4) (1,5) (2,6) (3,7) of a word of eight 4-bit values, minus their zero.  In fp16 the values at
+// bits 4..7 need no shift: 1024 + 16 q, times 1/16, minus 64 + zero, in one exact multiply-add (bf16's 7 mantissa bits
+// end below bit 7).
 template <bool kFp16>
 __device__ __forceinline__ void unpack_word(uint32_t w, uint32_t zp, uint32_t (&p)[4]) {
-  constexpr uint32_t kMagic = kFp16 ? 0x64006400u : 0x43004300u;
+  if constexpr (kFp16) {
+    const __half2 z = *reinterpret_cast<__half2*>(&zp);
+    const __half2 z16 = __hsub2(__half2half2(__float2half_rn(960.f)), z);  // -(64 + zero) = 960 - (1024 + zero)
+    const uint32_t w8 = w >> 8;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) p[i] = sub2<kFp16>(((w >> (4 * i)) & 0x000F000Fu) | kMagic, zp);
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t lo = and_or(i ? w8 : w, 0x000F000Fu, 0x64006400u), hi = and_or(i ? w8 : w, 0x00F000F0u, 0x64006400u);
+      const __half2 a = __hsub2(*reinterpret_cast<const __half2*>(&lo), z);
+      const __half2 b = __hfma2(*reinterpret_cast<const __half2*>(&hi), __half2half2(__float2half_rn(0.0625f)), z16);
+      p[2 * i] = *reinterpret_cast<const uint32_t*>(&a);
+      p[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&b);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = sub2<false>(and_or(w >> (4 * i), 0x000F000Fu, 0x43004300u), zp);
+  }
 }
 
-template <int kWN, int kWK, int kNT, int kStages>
+template <int kWN, int kWK, int kNT, int kStages, int kSB>
 struct W4Smem {
+  static constexpr int kWarps = kWN * kWK;         // that multiply; two more fetch
+  static constexpr int kThreads = (kWarps + 2) * 32;
   static constexpr int kRows = kWN * 32;
-  static constexpr int kWBytes = kRows * kW4RowBytes;
-  static constexpr int kStageBytes = kWBytes + kNT * 8 * kW4ABytes;
-  static constexpr int kRedPitch = kNT * 8 + 1;  // floats
-  static constexpr int kRedBytes = kWK * kRows * kRedPitch * 4;
-  static constexpr int kRing = kStages * kStageBytes > kRedBytes ? kStages * kStageBytes : kRedBytes;
-  static_assert(kWN * kWK * 32 == kW4Threads);
-  static_assert(kW4StageK / 32 % kWK == 0);
+  static constexpr int kWBytes = kRows * kSB * 16;
+  static constexpr int kStageBytes = kWBytes + kNT * 8 * kSB * 64;
+  static constexpr int kRedFloats = (kWK - 1) * kWN * 32 * 2 * kNT * 4;   // two buffers of them
+  static constexpr int kBarOffset = kStages * kStageBytes + 2 * kRedFloats * 4;
+  static constexpr int kBars = 2 * kStages + 4;
+  static constexpr int kScaleOffset = kBarOffset + (kBars * 8 + 15) / 16 * 16;
+  static_assert(kSB % 8 == 0 && kSB % (2 * kWK) == 0 && kStageBytes % 1024 == 0);
 };
 
-template <int kWN, int kWK, int kNT, int kStages, bool kGated, bool kFp16>
-__global__ void __launch_bounds__(kW4Threads, 2) w4_m_grouped_kernel(const W4Args p) {
-  using L = W4Smem<kWN, kWK, kNT, kStages>;
-  constexpr int kBlocks = kW4StageK / 32 / kWK;   // 32-wide k blocks of a stage that one warp multiplies
+template <int kWN, int kWK, int kNT, int kStages, int kSB, int kLogGs, bool kGated, bool kFp16>
+__global__ void __launch_bounds__(kWN * kWK * 32 + 64, kNT == 1 ? 2 : 1)
+w4_m_grouped_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_a, const W4Args p) {
+  using L = W4Smem<kWN, kWK, kNT, kStages, kSB>;
+  constexpr int kBlocks = kSB / kWK;                // 32-wide k blocks of a stage that one warp multiplies
+  constexpr int kPer = (1 << kLogGs) < kBlocks ? (1 << kLogGs) : kBlocks;   // of them under one scale
   constexpr int kOutCols = kGated ? L::kRows / 2 : L::kRows;
-  extern __shared__ __align__(128) uint8_t w4_smem[];
-  const uint32_t ring = smem_u32(w4_smem);
-  const uint32_t scales = ring + L::kRing;
-  const uint32_t zeros = scales + L::kRows * p.scale_pitch;
-  W4Expert* list = reinterpret_cast<W4Expert*>(w4_smem + L::kRing + L::kRows * (p.scale_pitch + p.zero_pitch));
-  __shared__ int s_active, s_items;
+  constexpr int kWindowStages = kW4WindowGroups * (1 << kLogGs) / kSB;      // stages that share a window of scales
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  const uint32_t smem_base = smem_u32(smem);
+  auto full_bar = [&](int s) { return smem_base + L::kBarOffset + 8u * s; };
+  auto empty_bar = [&](int s) { return smem_base + L::kBarOffset + 8u * (kStages + s); };
+  auto scale_full_bar = [&](int b) { return smem_base + L::kBarOffset + 8u * (2 * kStages + b); };
+  auto scale_empty_bar = [&](int b) { return smem_base + L::kBarOffset + 8u * (2 * kStages + 2 + b); };
+  const int scale_bytes = L::kRows * p.scale_pitch, staged_bytes = L::kRows * (p.scale_pitch + p.zero_pitch);
+  uint8_t* const staged = smem + L::kScaleOffset;   // two buffers of scales and zeros
+  W4Expert* const list = reinterpret_cast<W4Expert*>(staged + 2 * staged_bytes);
+  __shared__ int s_active, s_items, s_abort;
 
   const int tid = threadIdx.x;
-  const int warp = tid >> 5, lane = tid & 31;
-  const int wn = warp % kWN, wk = warp / kWN;
+  const int warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0), lane = tid & 31;
   const int weight_rows = kGated ? 2 * p.n : p.n;
-  const int groups = p.k >> (5 + p.log_gs32);
+  const int groups = p.k >> (5 + kLogGs);
   const int nblk = p.k >> 5;
-  const int stages = (nblk + 7) >> 3;
+  const int stages = (nblk + kSB - 1) / kSB;
+
+  if (tid == 32) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), L::kWarps);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(scale_full_bar(b), 32);
+      mbar_init(scale_empty_bar(b), L::kWarps);
+    }
+    s_abort = 0;
+    fence_mbar_init();
+    prefetch_tmap(&tm_w);
+    prefetch_tmap(&tm_a);
+  }
 
   // ---- the experts that have rows, in order, by one warp: lane i looks at expert 32 c + i
   if (warp == 0) {
     long long row = 0;   // rows before this chunk of experts
     int active = 0, items = 0;
     bool overflow = false;
+    constexpr int kAhead = 4;   // chunks whose sizes are on their way together
+    long long ahead[kAhead];
     for (int g0 = 0; g0 < p.num_groups; g0 += 32) {
+      const int which = (g0 >> 5) & (kAhead - 1);
+      if (which == 0) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          const int g = g0 + i * 32 + lane;
+          ahead[i] = 0;
+          if (g < p.num_groups)
+            ahead[i] = p.sizes_i64 ? static_cast<const long long*>(p.sizes)[g]
+                                   : static_cast<long long>(static_cast<const int*>(p.sizes)[g]);
+        }
+      }
       const int g = g0 + lane;
-      long long v = 0;
-      if (g < p.num_groups)
-        v = p.sizes_i64 ? static_cast<const long long*>(p.sizes)[g]
-                        : static_cast<long long>(static_cast<const int*>(p.sizes)[g]);
+      long long v = which == 0 ? ahead[0] : which == 1 ? ahead[1] : which == 2 ? ahead[2] : ahead[3];
       if (v < 0) v = 0;
       if (v > p.m_rows) {   // cut off below, like every M-grouped entry point; keeps the sums in range
         v = p.m_rows;
@@ -223,7 +254,10 @@ __global__ void __launch_bounds__(kW4Threads, 2) w4_m_grouped_kernel(const W4Arg
   __syncthreads();
   const int active = s_active, items = s_items;
 
-  for (int item = blockIdx.x; item < items; item += gridDim.x) {
+  struct Item {
+    int g, row0, rows, n0;
+  };
+  auto item_at = [&](int item) {
     int lo = 0, hi = active - 1;
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
@@ -234,144 +268,165 @@ __global__ void __launch_bounds__(kW4Threads, 2) w4_m_grouped_kernel(const W4Arg
     const int chunks = (e.rows + kNT * 8 - 1) / (kNT * 8);
     const int tile = (item - e.item0) / chunks;
     const int chunk = (item - e.item0) - tile * chunks;
-    const int row0 = e.row0 + chunk * kNT * 8;
-    const int rows = min(kNT * 8, e.rows - chunk * kNT * 8);
-    const int nt_used = (rows + 7) >> 3;
-    const int n0 = tile * kOutCols;
-    // weight row of tile row i: warps own 32 tile rows each; gated: 16 gate rows, then the 16 up rows of the same
-    // outputs.  Rows past the end are read from the last one and their results dropped.
-    auto weight_row = [&](int i) -> long long {
-      long long r;
-      if constexpr (kGated) {
-        const int col = min(n0 + (i >> 5) * 16 + (i & 15), p.n - 1);
-        r = (i & 16) ? p.n + col : col;
-      } else {
-        r = min(n0 + i, p.n - 1);
-      }
-      return static_cast<long long>(e.g) * weight_rows + r;
-    };
+    return Item{e.g, e.row0 + chunk * kNT * 8, min(kNT * 8, e.rows - chunk * kNT * 8), tile * kOutCols};
+  };
 
-    // this thread's pieces of a stage: weight rows (tid / 8) + 32 i, 16-byte column tid % 8; rows of `a` likewise
-    const int w_col = tid & 7;
-    const uint8_t* w_src[L::kRows / 32];
+  if (warp == L::kWarps) {
+    // ---- the stages of this block's items, by one thread
+    if (lane == 0) {
+      int slot = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int item = blockIdx.x; ok && item < items; item += gridDim.x) {
+        const Item it = item_at(item);
+        for (int st = 0; st < stages; ++st) {
+          if (!wait_bounded(empty_bar(slot), phase ^ 1u, &s_abort, p.status, kDevTimeoutProducer)) {
+            ok = false;
+            break;
+          }
+          const uint32_t bar = full_bar(slot), w_dst = smem_base + slot * L::kStageBytes, a_dst = w_dst + L::kWBytes;
+          mbar_arrive_expect_tx(bar, L::kStageBytes);
 #pragma unroll
-    for (int i = 0; i < L::kRows / 32; ++i)
-      w_src[i] = p.w + weight_row((tid >> 3) + 32 * i) * (p.k >> 1) + w_col * 16;
-    const uint8_t* a_src = p.a + static_cast<long long>(row0) * p.k * 2;
-
-    auto fetch = [&](int st) {
-      const uint32_t base = ring + (st % kStages) * L::kStageBytes;
-      if (st * 8 + w_col < nblk) {
+          for (int i = 0; i < kSB / 8; ++i) {   // 128 bytes of every row; past the end of a dimension zeros come in
+            const uint32_t d = w_dst + i * L::kRows * 128;
+            const int x = st * (kSB * 16) + i * 128;
+            tma_load_4d(d, &tm_w, bar, x, it.n0, 0, it.g);
+            if constexpr (kGated) tma_load_4d(d + L::kRows * 64, &tm_w, bar, x, it.n0, 1, it.g);
+          }
 #pragma unroll
-        for (int i = 0; i < L::kRows / 32; ++i)
-          cp_async16(base + ((tid >> 3) + 32 * i) * kW4RowBytes + w_col * 16, w_src[i] + static_cast<long long>(st) * 128);
-      }
-      // `a`: 32 16-byte columns per row and stage, a warp per row
-      const int col = st * 32 + lane;
-      if (col * 8 < p.k) {
-        for (int r = warp; r < rows; r += kW4Threads / 32)
-          cp_async16(base + L::kWBytes + r * kW4ABytes + lane * 16, a_src + static_cast<long long>(r) * p.k * 2 + col * 16);
-      }
-    };
-    // scales and zeros of the groups [first, first + count) of the tile's rows
-    auto fetch_scales = [&](int first) {
-      const int count = min(kW4WindowGroups, groups - first);
-      for (int r = warp; r < L::kRows; r += kW4Threads / 32) {
-        const long long at = weight_row(r) * groups + first;
-        const uint8_t* s = p.scale + at * 2;
-        const uint32_t d = scales + r * p.scale_pitch;
-        if (((reinterpret_cast<uintptr_t>(s) | (count * 2)) & 15) == 0) {
-          for (int c = lane; c < count / 8; c += 32) cp_async16(d + c * 16, s + c * 16);
-        } else {
-          for (int c = lane; c < count; c += 32)
-            asm volatile("st.shared.b16 [%0], %1;" ::"r"(d + c * 2), "h"(reinterpret_cast<const uint16_t*>(s)[c]) : "memory");
-        }
-        if (p.zero) {
-          const uint8_t* z = p.zero + at;
-          const uint32_t dz = zeros + r * p.zero_pitch;
-          if (((reinterpret_cast<uintptr_t>(z) | count) & 15) == 0) {
-            for (int c = lane; c < count / 16; c += 32) cp_async16(dz + c * 16, z + c * 16);
-          } else {
-            for (int c = lane; c < count; c += 32)
-              asm volatile("st.shared.u8 [%0], %1;" ::"r"(dz + c), "r"(static_cast<uint32_t>(z[c])) : "memory");
+          for (int i = 0; i < kSB / 2; ++i)
+            tma_load_2d(a_dst + i * kNT * 1024, &tm_a, bar, st * (kSB * 32) + i * 64, it.row0);
+          if (++slot == kStages) {
+            slot = 0;
+            phase ^= 1u;
           }
         }
       }
-    };
-
-    float acc[2][kNT][4], part[2][kNT][4];
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int j = 0; j < kNT; ++j)
-#pragma unroll
-        for (int v = 0; v < 4; ++v) acc[i][j][v] = part[i][j][v] = 0.f;
-
-#pragma unroll
-    for (int s = 0; s < kStages - 1; ++s) {
-      if (s < stages) fetch(s);
-      if (s == 0) fetch_scales(0);
-      cp_async_commit();
     }
-
-    const int lr = lane >> 2, lt = lane & 3;
-    int window = 0;  // first group of the staged scales
-    uint32_t zp[2][2] = {{zero_pair<kFp16>(8), zero_pair<kFp16>(8)}, {zero_pair<kFp16>(8), zero_pair<kFp16>(8)}};
-    for (int st = 0; st < stages; ++st) {
-      cp_async_wait<kStages - 2>();
-      __syncthreads();   // stage st has landed for everybody, and everybody is done with stage st - 1
-      if (const int g = (st * 8) >> p.log_gs32; g - window >= kW4WindowGroups) {
-        window = g;
-        fetch_scales(g);
-        cp_async_commit();
-        cp_async_wait<0>();
-        __syncthreads();
+  } else if (warp == L::kWarps + 1) {
+    // ---- the scales and zeros of this block's items, kW4WindowGroups groups at a time, by one warp.  Tile row r: gated:
+    // gate rows, then the up rows of the same outputs; rows past the end are read from the last one.
+    uint32_t use = 0;
+    bool ok = true;
+    for (int item = blockIdx.x; ok && item < items; item += gridDim.x) {
+      const Item it = item_at(item);
+      for (int first = 0; first < groups; first += kW4WindowGroups, ++use) {
+        const int buf = use & 1u;
+        if (!wait_bounded(scale_empty_bar(buf), ((use >> 1) & 1u) ^ 1u, &s_abort, p.status, kDevTimeoutProducer)) {
+          ok = false;
+          break;
+        }
+        const int count = min(kW4WindowGroups, groups - first);
+        uint8_t* const base = staged + buf * staged_bytes;
+        auto row_at = [&](int r) {
+          const int col = min(it.n0 + (kGated ? r % kOutCols : r), p.n - 1);
+          return (static_cast<long long>(it.g) * weight_rows + (kGated && r >= kOutCols ? p.n + col : col)) * groups + first;
+        };
+        for (int i = lane; i < L::kRows << p.log_scale_vecs; i += 32) {
+          const int r = i >> p.log_scale_vecs, v = (i & ((1 << p.log_scale_vecs) - 1)) * 8;   // 8 scales
+          if (v >= count) continue;
+          const uint16_t* s = reinterpret_cast<const uint16_t*>(p.scale) + row_at(r) + v;
+          uint8_t* d = base + r * p.scale_pitch + v * 2;
+          if (v + 8 <= count && (reinterpret_cast<uintptr_t>(s) & 15) == 0) cp_async16(smem_u32(d), s);
+          else
+            for (int c = 0; c < min(8, count - v); ++c) reinterpret_cast<uint16_t*>(d)[c] = s[c];
+        }
+        if (p.zero) {
+          for (int i = lane; i < L::kRows << p.log_zero_vecs; i += 32) {
+            const int r = i >> p.log_zero_vecs, v = (i & ((1 << p.log_zero_vecs) - 1)) * 16;
+            if (v >= count) continue;
+            const uint8_t* z = p.zero + row_at(r) + v;
+            uint8_t* d = base + scale_bytes + r * p.zero_pitch + v;
+            if (v + 16 <= count && (reinterpret_cast<uintptr_t>(z) & 15) == 0) cp_async16(smem_u32(d), z);
+            else
+              for (int c = 0; c < min(16, count - v); ++c) d[c] = z[c];
+          }
+        }
+        cp_async_wait_all();
+        mbar_arrive(scale_full_bar(buf));   // every lane: its own copies and stores are done
       }
-      if (st + kStages - 1 < stages) fetch(st + kStages - 1);
-      cp_async_commit();
-
-      const uint32_t base = ring + (st % kStages) * L::kStageBytes;
-      const uint32_t w_row = base + (wn * 32 + lr) * kW4RowBytes + lt * 4;
-      const uint32_t a_row = base + L::kWBytes + lr * kW4ABytes + lt * 16;
+    }
+  } else {
+    // ---- multiplication
+    const int wn = warp % kWN, wk = warp / kWN;
+    const int lr = lane >> 2, lt = lane & 3;
+    // fragment addresses inside a stage: weight row (its 8-row group's row lr), k block wk * kBlocks + b
+    auto tile_row = [&](int i) { return kGated ? i * kOutCols + wn * 16 : wn * 32 + i * 16; };
+    uint32_t w_off[kBlocks];
 #pragma unroll
-      for (int b = 0; b < kBlocks; ++b) {
-        const int in_stage = wk * kBlocks + b;
-        const int blk = st * 8 + in_stage;
-        if (blk >= nblk) break;
-        const int grp = (blk >> p.log_gs32) - window;
-        if (p.zero && (b == 0 || (blk & ((1 << p.log_gs32) - 1)) == 0)) {
+    for (int b = 0; b < kBlocks; ++b) {
+      const int c = wk * kBlocks + b;
+      w_off[b] = (c >> 3) * (L::kRows * 128) + lr * 128 + (((c & 7) ^ lr) << 4) + lt * 4;
+    }
+    const int a_row = (lr >> 1) + 4 * (lr & 1);   // the row of `a` in column lr of a product
+    uint32_t a_off[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      a_off[h] = L::kWBytes + wk * (kBlocks / 2) * kNT * 1024 + a_row * 128 + (((h * 4 + lt) ^ a_row) << 4);
+    float* const red = reinterpret_cast<float*>(smem + kStages * L::kStageBytes);
+
+    int slot = 0;
+    uint32_t phase = 0, use = 0;
+    int red_buf = 0;
+    bool ok = true;   // false: a wait ran out; the rest is walked through without touching data
+    for (int item = blockIdx.x; item < items; item += gridDim.x, red_buf ^= 1) {
+      const Item it = item_at(item);
+      const int nt_used = (it.rows + 7) >> 3;
+      float acc[2][kNT][4];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < kNT; ++j)
+#pragma unroll
+          for (int v = 0; v < 4; ++v) acc[i][j][v] = 0.f;
+
+      // blocks [0, valid) of this warp's part of the stage in `slot`; grp0: staged group of the first
+      auto multiply = [&](auto with_zero, auto whole, int grp0, int valid) {
+        constexpr bool kZero = decltype(with_zero)::value, kWhole = decltype(whole)::value;
+        const uint8_t* const st = smem + slot * L::kStageBytes;
+        const uint8_t* const s_frag = staged + (use & 1u) * staged_bytes + lr * p.scale_pitch;
+        const uint8_t* const z_frag = staged + (use & 1u) * staged_bytes + scale_bytes + lr * p.zero_pitch;
+#pragma unroll
+        for (int b0 = 0; b0 < kBlocks; b0 += kPer) {
+          if (!kWhole && b0 >= valid) break;   // k is a multiple of the group: a started run of kPer blocks is whole
+          const int grp = grp0 + (b0 >> kLogGs);
+          uint32_t zp[2][2];
 #pragma unroll
           for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int h = 0; h < 2; ++h)
-              zp[i][h] = zero_pair<kFp16>(lds8(zeros + (wn * 32 + i * 16 + h * 8 + lr) * p.zero_pitch + grp));
-        }
-        uint32_t wv[2][2][4];
+              zp[i][h] = zero_pair<kFp16>(kZero ? z_frag[(tile_row(i) + h * 8) * p.zero_pitch + grp] : 8u);
+          float part[2][kNT][4];
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+          for (int b = b0; b < b0 + kPer; ++b) {
+            uint32_t wv[2][2][4];
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
-            unpack_word<kFp16>(lds32(w_row + (i * 16 + h * 8) * kW4RowBytes + in_stage * 16), zp[i][h], wv[i][h]);
+            for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int j = 0; j < kNT; ++j) {
-          if (kNT > 1 && j >= nt_used) break;
-          const uint4 q = lds128(a_row + j * 8 * kW4ABytes + in_stage * 64);
-          const uint32_t x04 = __byte_perm(q.x, q.z, 0x5410), x15 = __byte_perm(q.x, q.z, 0x7632);
-          const uint32_t x26 = __byte_perm(q.y, q.w, 0x5410), x37 = __byte_perm(q.y, q.w, 0x7632);
+              for (int h = 0; h < 2; ++h)
+                unpack_word<kFp16>(*reinterpret_cast<const uint32_t*>(st + w_off[b] + (tile_row(i) + h * 8) * 128), zp[i][h],
+                                   wv[i][h]);
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const uint32_t f0[4] = {wv[i][0][0], wv[i][1][0], wv[i][0][1], wv[i][1][1]};
-            const uint32_t f1[4] = {wv[i][0][2], wv[i][1][2], wv[i][0][3], wv[i][1][3]};
-            mma_16816<kFp16>(part[i][j], f0, x04, x15);
-            mma_16816<kFp16>(part[i][j], f1, x26, x37);
+            for (int j = 0; j < kNT; ++j) {
+              if (kNT > 1 && j >= nt_used) break;
+              const uint4 q = *reinterpret_cast<const uint4*>(st + a_off[b & 1] + (b >> 1) * kNT * 1024 + j * 1024);
+              const uint32_t x04 = __byte_perm(q.x, q.z, 0x5410), x15 = __byte_perm(q.x, q.z, 0x7632);
+              const uint32_t x26 = __byte_perm(q.y, q.w, 0x5410), x37 = __byte_perm(q.y, q.w, 0x7632);
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const uint32_t f0[4] = {wv[i][0][0], wv[i][1][0], wv[i][0][1], wv[i][1][1]};
+                const uint32_t f1[4] = {wv[i][0][2], wv[i][1][2], wv[i][0][3], wv[i][1][3]};
+                if (b == b0) mma_16816<kFp16, true>(part[i][j], f0, x04, x15);
+                else mma_16816<kFp16, false>(part[i][j], f0, x04, x15);
+                mma_16816<kFp16, false>(part[i][j], f1, x26, x37);
+              }
+            }
           }
-        }
-        // the last block of a group, or of what this warp has of it: the scale enters
-        if (b == kBlocks - 1 || blk + 1 == nblk || ((blk + 1) & ((1 << p.log_gs32) - 1)) == 0) {
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const uint32_t sa = scales + (wn * 32 + i * 16 + lr) * p.scale_pitch + grp * 2;
-            const float s0 = to_float<kFp16>(lds16(sa)), s1 = to_float<kFp16>(lds16(sa + 8 * p.scale_pitch));
+            const uint8_t* sa = s_frag + tile_row(i) * p.scale_pitch + grp * 2;
+            const float s0 = to_float<kFp16>(*reinterpret_cast<const uint16_t*>(sa));
+            const float s1 = to_float<kFp16>(*reinterpret_cast<const uint16_t*>(sa + 8 * p.scale_pitch));
 #pragma unroll
             for (int j = 0; j < kNT; ++j) {
               if (kNT > 1 && j >= nt_used) break;
@@ -379,54 +434,89 @@ __global__ void __launch_bounds__(kW4Threads, 2) w4_m_grouped_kernel(const W4Arg
               acc[i][j][1] = fmaf(s0, part[i][j][1], acc[i][j][1]);
               acc[i][j][2] = fmaf(s1, part[i][j][2], acc[i][j][2]);
               acc[i][j][3] = fmaf(s1, part[i][j][3], acc[i][j][3]);
+            }
+          }
+        }
+      };
+
+      for (int st0 = 0; st0 < stages; st0 += kWindowStages, ++use) {
+        ok = ok && wait_bounded(scale_full_bar(use & 1u), (use >> 1) & 1u, &s_abort, p.status, kDevTimeoutMma);
+        const int st_end = min(stages, st0 + kWindowStages);
+        for (int st = st0; st < st_end; ++st) {
+          ok = ok && wait_bounded(full_bar(slot), phase, &s_abort, p.status, kDevTimeoutMma);
+          if (!ok) continue;
+          const int grp0 = ((st - st0) * kSB + wk * kBlocks) >> kLogGs;
+          if ((st + 1) * kSB <= nblk) {
+            if (p.zero) multiply(std::true_type{}, std::true_type{}, grp0, kBlocks);
+            else multiply(std::false_type{}, std::true_type{}, grp0, kBlocks);
+          } else {
+            const int valid = nblk - st * kSB - wk * kBlocks;
+            if (p.zero) multiply(std::true_type{}, std::false_type{}, grp0, valid);
+            else multiply(std::false_type{}, std::false_type{}, grp0, valid);
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(empty_bar(slot));
+          if (++slot == kStages) {
+            slot = 0;
+            phase ^= 1u;
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(scale_empty_bar(use & 1u));
+      }
+
+      // ---- join the kWK partial sums (in order) and store.  Every warp holds its values in the same lanes; the two
+      // buffers alternate, so one meeting per item is enough.
+      float* const joined = red + red_buf * L::kRedFloats + wn * (2 * kNT * 4) * 32 + lane;
+      constexpr int kWarpStep = kWN * (2 * kNT * 4) * 32;
+      if (wk > 0) {
 #pragma unroll
-              for (int v = 0; v < 4; ++v) part[i][j][v] = 0.f;
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < kNT; ++j) {
+            if (kNT > 1 && j >= nt_used) break;
+#pragma unroll
+            for (int v = 0; v < 4; ++v) joined[(wk - 1) * kWarpStep + ((i * kNT + j) * 4 + v) * 32] = acc[i][j][v];
+          }
+      }
+      asm volatile("bar.sync 1, %0;" ::"n"(L::kWarps * 32) : "memory");
+      if (wk == 0 && ok) {
+#pragma unroll
+        for (int j = 0; j < kNT; ++j) {
+          if (kNT > 1 && j >= nt_used) break;
+#pragma unroll
+          for (int q = 1; q < kWK; ++q)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int v = 0; v < 4; ++v) acc[i][j][v] += joined[(q - 1) * kWarpStep + ((i * kNT + j) * 4 + v) * 32];
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            const int r = j * 8 + lt + (v & 1) * 4;     // column 2 lt + (v & 1) of the product
+            if (r >= it.rows) continue;
+            uint16_t* out = p.out + static_cast<long long>(it.row0 + r) * p.n;
+            auto store = [&](int col, float value) {
+              if (col >= p.n) return;
+              if constexpr (kFp16) out[col] = __half_as_ushort(__float2half_rn(value));
+              else out[col] = __bfloat16_as_ushort(__float2bfloat16_rn(value));
+            };
+            const int c = lr + (v >> 1) * 8;            // row inside the warp's 16
+            if constexpr (kGated) {
+              const float g = acc[0][j][v];
+              store(it.n0 + wn * 16 + c,
+                    (p.act == kActSilu ? gate_value<kActSilu>(g) : gate_value<kActGeluTanh>(g)) * acc[1][j][v]);
+            } else {
+              store(it.n0 + wn * 32 + c, acc[0][j][v]);
+              store(it.n0 + wn * 32 + 16 + c, acc[1][j][v]);
             }
           }
         }
       }
     }
-
-    // ---- join the kWK partial sums (in order) and store
-    cp_async_wait<0>();
-    __syncthreads();
-    float* red = reinterpret_cast<float*>(w4_smem);
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int j = 0; j < kNT; ++j) {
-        if (kNT > 1 && j >= nt_used) break;
-        float* d = red + ((wk * kWN + wn) * 32 + i * 16 + lr) * L::kRedPitch + j * 8 + lt * 2;
-        d[0] = acc[i][j][0];
-        d[1] = acc[i][j][1];
-        d[8 * L::kRedPitch] = acc[i][j][2];
-        d[8 * L::kRedPitch + 1] = acc[i][j][3];
-      }
-    __syncthreads();
-    for (int o = tid; o < kOutCols * rows; o += kW4Threads) {
-      const int r = o / kOutCols;          // a power of two: a shift
-      const int c = o - r * kOutCols;
-      if (n0 + c >= p.n) continue;
-      auto joined = [&](int tile_row) {
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < kWK; ++i) s += red[(i * L::kRows + tile_row) * L::kRedPitch + r];
-        return s;
-      };
-      float v;
-      if constexpr (kGated) {
-        const int tr = (c >> 4) * 32 + (c & 15);
-        v = gate_value(joined(tr), p.act) * joined(tr + 16);
-      } else {
-        v = joined(c);
-      }
-      uint16_t bits;
-      if constexpr (kFp16) bits = __half_as_ushort(__float2half_rn(v));
-      else bits = __bfloat16_as_ushort(__float2bfloat16_rn(v));
-      p.out[static_cast<long long>(row0 + r) * p.n + n0 + c] = bits;
-    }
-    __syncthreads();  // the ring and the staged scales are free again
   }
+  __syncthreads();
+  if (*static_cast<volatile int*>(&s_abort))
+    for (int i = 0; i < 64; ++i) __nanosleep(4000);   // copies still in flight land before the memory goes
 }
 
 // ------------------------------------------------------------------ quantiser
@@ -486,24 +576,58 @@ w4_quant_kernel(const uint16_t* __restrict__ w, uint8_t* __restrict__ q, uint16_
 }
 
 // ------------------------------------------------------------------ host side
-template <int kWN, int kWK, int kNT, int kStages, bool kGated, bool kFp16>
-static int launch_w4(W4Args p, int want_sms, cudaStream_t stream) {
-  using L = W4Smem<kWN, kWK, kNT, kStages>;
-  auto kern = w4_m_grouped_kernel<kWN, kWK, kNT, kStages, kGated, kFp16>;
+struct W4Operands {
+  const void* a;
+  const void* w;
+};
+
+template <int kWN, int kWK, int kNT, int kStages, int kSB, int kLogGs, bool kGated, bool kFp16>
+static int launch_w4(const W4Operands& o, W4Args p, int want_sms, cudaStream_t stream) {
+  using L = W4Smem<kWN, kWK, kNT, kStages, kSB>;
+  static_assert((kW4WindowGroups << kLogGs) % kSB == 0, "a window ends with a stage");
+  auto kern = w4_m_grouped_kernel<kWN, kWK, kNT, kStages, kSB, kLogGs, kGated, kFp16>;
   constexpr int kOutCols = kGated ? L::kRows / 2 : L::kRows;
   p.tiles = (p.n + kOutCols - 1) / kOutCols;
-  const int smem = L::kRing + L::kRows * (p.scale_pitch + p.zero_pitch) +
-                   p.list_capacity * static_cast<int>(sizeof(W4Expert));
+  const int smem = L::kScaleOffset + 2 * L::kRows * (p.scale_pitch + p.zero_pitch) +
+                   p.list_capacity * static_cast<int>(sizeof(W4Expert)) + 1024;
+  CUtensorMap tm_w, tm_a;
+  {
+    const uint64_t row = static_cast<uint64_t>(p.k) / 2, n = static_cast<uint64_t>(p.n), halves = kGated ? 2 : 1;
+    const uint64_t dims[4] = {row, n, halves, static_cast<uint64_t>(p.num_groups)};
+    const uint64_t strides[3] = {row, row * n, row * n * halves};
+    const uint32_t box[4] = {128, static_cast<uint32_t>(kOutCols), 1, 1};
+    if (int rc = encode_tmap(&tm_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, o.w, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B,
+                             "W4[G,N,K/2]"))
+      return rc;
+  }
+  {
+    const uint64_t dims[2] = {static_cast<uint64_t>(p.k), static_cast<uint64_t>(p.m_rows)};
+    const uint64_t strides[1] = {static_cast<uint64_t>(p.k) * 2};
+    const uint32_t box[2] = {64, kNT * 8};
+    if (int rc = encode_tmap(&tm_a, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, o.a, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, "A"))
+      return rc;
+  }
   B200_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  const int per_sm = 2 * (smem + 2048) <= 228 * 1024 ? 2 : 1;  // the registers allow two
+  const int per_sm = kNT == 1 && 2 * (smem + 2048) <= 228 * 1024 ? 2 : 1;
   // at most this many items: every expert with rows has one partial chunk at most
   const long long chunks = p.m_rows / (kNT * 8) + (p.m_rows < p.num_groups ? p.m_rows : p.num_groups);
   const long long items = chunks * p.tiles;
-  B200_REQUIRE(items < (1ll << 31), "b200gemm_w4_m_grouped: too many rows and columns for one call");
+  B200_REQUIRE(items < (1ll << 31) - 65536, "b200gemm_w4_m_grouped: too many rows and columns for one call");
   const long long resident = static_cast<long long>(per_sm) * want_sms;
-  kern<<<static_cast<unsigned>(items < resident ? items : resident), kW4Threads, smem, stream>>>(p);
+  kern<<<static_cast<unsigned>(items < resident ? items : resident), L::kThreads, smem, stream>>>(tm_w, tm_a, p);
   B200_CUDA(cudaGetLastError());
   return 0;
+}
+
+template <int kWN, int kWK, int kNT, int kStages, int kSB>
+static int form_w4(const W4Operands& o, const W4Args& p, int log_gs, int gated, int dtype, int want_sms, cudaStream_t stream) {
+#define B200_W4(GS, GATED, FP16) launch_w4<kWN, kWK, kNT, kStages, kSB, GS, GATED, FP16>(o, p, want_sms, stream)
+#define B200_W4_GS(GATED, FP16) \
+  (log_gs == 0 ? B200_W4(0, GATED, FP16) : log_gs == 1 ? B200_W4(1, GATED, FP16) : B200_W4(2, GATED, FP16))
+  return gated ? (dtype ? B200_W4_GS(true, true) : B200_W4_GS(true, false))
+               : (dtype ? B200_W4_GS(false, true) : B200_W4_GS(false, false));
+#undef B200_W4_GS
+#undef B200_W4
 }
 
 static int w4_m_grouped(const void* a, const void* w4, const void* scale, const void* zero, void* out, const void* sizes,
@@ -528,8 +652,6 @@ static int w4_m_grouped(const void* a, const void* w4, const void* scale, const 
   const int sms = sm_count();
   B200_REQUIRE(sms > 0, "%s: no CUDA device", who);
   W4Args p = {};
-  p.a = static_cast<const uint8_t*>(a);
-  p.w = static_cast<const uint8_t*>(w4);
   p.scale = static_cast<const uint8_t*>(scale);
   p.zero = static_cast<const uint8_t*>(zero);
   p.out = static_cast<uint16_t*>(out);
@@ -539,23 +661,20 @@ static int w4_m_grouped(const void* a, const void* w4, const void* scale, const 
   p.m_rows = m_rows;
   p.n = n;
   p.k = k;
-  p.log_gs32 = group_size == 32 ? 0 : group_size == 64 ? 1 : 2;
   p.act = act;
   const int groups = k / group_size;
   const int window = groups < kW4WindowGroups ? groups : kW4WindowGroups;
-  p.scale_pitch = ((window * 2 + 15) / 16 | 1) * 16;   // an odd number of 16-byte units: 8 rows, 8 different banks
+  p.scale_pitch = ((window * 2 + 15) / 16 | 1) * 16;
   p.zero_pitch = zero ? ((window + 15) / 16 | 1) * 16 : 0;
+  p.log_scale_vecs = window <= 8 ? 0 : window <= 16 ? 1 : 2;
+  p.log_zero_vecs = window <= 16 ? 0 : 1;
   p.list_capacity = static_cast<int>(m_rows < num_groups ? m_rows : num_groups);
   p.status = device_status_ptr();
   const int want = num_sms > 0 && num_sms < sms ? num_sms : sms;
-#define B200_W4(WN, WK, NT, ST)                                                          \
-  (gated ? (dtype ? launch_w4<WN, WK, NT, ST, true, true>(p, want, stream)               \
-                  : launch_w4<WN, WK, NT, ST, true, false>(p, want, stream))             \
-         : (dtype ? launch_w4<WN, WK, NT, ST, false, true>(p, want, stream)              \
-                  : launch_w4<WN, WK, NT, ST, false, false>(p, want, stream)))
-  if (m_rows <= 8) return B200_W4(2, 4, 1, 4);
-  return B200_W4(4, 2, 4, 3);
-#undef B200_W4
+  const int log_gs = group_size == 32 ? 0 : group_size == 64 ? 1 : 2;
+  const W4Operands o = {a, w4};
+  return m_rows <= 8ll * num_groups ? form_w4<2, 4, 1, 3, 16>(o, p, log_gs, gated, dtype, want, stream)
+                                    : form_w4<4, 2, 4, 4, 8>(o, p, log_gs, gated, dtype, want, stream);
 }
 
 static int w4_quant(const void* w, void* q, void* scale, void* zero, int64_t rows, int k, int group_size, int dtype,
