@@ -78,6 +78,24 @@ __device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t parity, vola
   return true;
 }
 
+// Same for a role that has nothing else to do and shares its scheduler with warps that compute: the hardware
+// parks the thread for up to 20 us per attempt instead of the default, so it issues next to nothing.
+__device__ __forceinline__ bool wait_bounded_parked(uint32_t bar, uint32_t parity, volatile int* abort_flag,
+                                                    unsigned* status, unsigned role_bit) {
+  uint64_t t0 = 0;
+  while (!mbar_try_wait_parked(bar, parity, 20000)) {
+    if (*abort_flag) return false;
+    const uint64_t now = global_timer_ns();
+    if (t0 == 0) t0 = now;
+    if (now - t0 > kWaitLimitNs) {
+      *abort_flag = 1;
+      if (status) atomicOr(status, role_bit);
+      return false;
+    }
+  }
+  return true;
+}
+
 // Polling variant (mbarrier.test_wait, no hardware suspend) for handshakes whose wake-up
 // latency is on the critical path; same bound, same abort protocol.
 __device__ __forceinline__ bool wait_bounded_spin(uint32_t bar, uint32_t parity, volatile int* abort_flag,

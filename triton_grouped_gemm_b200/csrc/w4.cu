@@ -36,6 +36,8 @@
 namespace b200 {
 
 constexpr int kW4WindowGroups = 32;   // scales are staged for this many groups at a time
+constexpr int kW4ScalePitch = 80;     // bytes per row of the staged scales / zeros: odd numbers of 16-byte units,
+constexpr int kW4ZeroPitch = 48;      // so that 8 rows lie in 8 different banks
 constexpr int kW4MaxGroups = 1024;    // experts
 
 struct W4Args {
@@ -49,8 +51,6 @@ struct W4Args {
   int n, k;
   int act;
   int tiles;             // tiles per expert
-  int scale_pitch;       // bytes per row of the staged scales / zeros: odd numbers of 16-byte units, conflict-free
-  int zero_pitch;
   int log_scale_vecs;    // log2 of the 16-byte pieces (rounded up to a power of two) of a row's staged scales / zeros
   int log_zero_vecs;
   int list_capacity;     // entries of the list of experts with rows
@@ -138,6 +138,8 @@ struct W4Smem {
   static constexpr int kWarps = kWN * kWK;         // that multiply; two more fetch
   static constexpr int kThreads = (kWarps + 2) * 32;
   static constexpr int kRows = kWN * 32;
+  static constexpr int kScaleBytes = kRows * kW4ScalePitch;
+  static constexpr int kStagedBytes = kRows * (kW4ScalePitch + kW4ZeroPitch);
   static constexpr int kWBytes = kRows * kSB * 16;
   static constexpr int kStageBytes = kWBytes + kNT * 8 * kSB * 64;
   static constexpr int kRedFloats = (kWK - 1) * kWN * 32 * 2 * kNT * 4;   // two buffers of them
@@ -147,7 +149,7 @@ struct W4Smem {
   static_assert(kSB % 8 == 0 && kSB % (2 * kWK) == 0 && kStageBytes % 1024 == 0);
 };
 
-template <int kWN, int kWK, int kNT, int kStages, int kSB, int kLogGs, bool kGated, bool kFp16>
+template <int kWN, int kWK, int kNT, int kStages, int kSB, int kLogGs, bool kGated, bool kFp16, bool kZero>
 __global__ void __launch_bounds__(kWN * kWK * 32 + 64, kNT == 1 ? 2 : 1)
 w4_m_grouped_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_a, const W4Args p) {
   using L = W4Smem<kWN, kWK, kNT, kStages, kSB>;
@@ -162,9 +164,8 @@ w4_m_grouped_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
   auto empty_bar = [&](int s) { return smem_base + L::kBarOffset + 8u * (kStages + s); };
   auto scale_full_bar = [&](int b) { return smem_base + L::kBarOffset + 8u * (2 * kStages + b); };
   auto scale_empty_bar = [&](int b) { return smem_base + L::kBarOffset + 8u * (2 * kStages + 2 + b); };
-  const int scale_bytes = L::kRows * p.scale_pitch, staged_bytes = L::kRows * (p.scale_pitch + p.zero_pitch);
   uint8_t* const staged = smem + L::kScaleOffset;   // two buffers of scales and zeros
-  W4Expert* const list = reinterpret_cast<W4Expert*>(staged + 2 * staged_bytes);
+  W4Expert* const list = reinterpret_cast<W4Expert*>(staged + 2 * L::kStagedBytes);
   __shared__ int s_active, s_items, s_abort;
 
   const int tid = threadIdx.x;
@@ -280,7 +281,7 @@ w4_m_grouped_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
       for (int item = blockIdx.x; ok && item < items; item += gridDim.x) {
         const Item it = item_at(item);
         for (int st = 0; st < stages; ++st) {
-          if (!wait_bounded(empty_bar(slot), phase ^ 1u, &s_abort, p.status, kDevTimeoutProducer)) {
+          if (!wait_bounded_parked(empty_bar(slot), phase ^ 1u, &s_abort, p.status, kDevTimeoutProducer)) {
             ok = false;
             break;
           }
@@ -312,12 +313,12 @@ w4_m_grouped_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
       const Item it = item_at(item);
       for (int first = 0; first < groups; first += kW4WindowGroups, ++use) {
         const int buf = use & 1u;
-        if (!wait_bounded(scale_empty_bar(buf), ((use >> 1) & 1u) ^ 1u, &s_abort, p.status, kDevTimeoutProducer)) {
+        if (!wait_bounded_parked(scale_empty_bar(buf), ((use >> 1) & 1u) ^ 1u, &s_abort, p.status, kDevTimeoutProducer)) {
           ok = false;
           break;
         }
         const int count = min(kW4WindowGroups, groups - first);
-        uint8_t* const base = staged + buf * staged_bytes;
+        uint8_t* const base = staged + buf * L::kStagedBytes;
         auto row_at = [&](int r) {
           const int col = min(it.n0 + (kGated ? r % kOutCols : r), p.n - 1);
           return (static_cast<long long>(it.g) * weight_rows + (kGated && r >= kOutCols ? p.n + col : col)) * groups + first;
@@ -326,17 +327,17 @@ w4_m_grouped_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
           const int r = i >> p.log_scale_vecs, v = (i & ((1 << p.log_scale_vecs) - 1)) * 8;   // 8 scales
           if (v >= count) continue;
           const uint16_t* s = reinterpret_cast<const uint16_t*>(p.scale) + row_at(r) + v;
-          uint8_t* d = base + r * p.scale_pitch + v * 2;
+          uint8_t* d = base + r * kW4ScalePitch + v * 2;
           if (v + 8 <= count && (reinterpret_cast<uintptr_t>(s) & 15) == 0) cp_async16(smem_u32(d), s);
           else
             for (int c = 0; c < min(8, count - v); ++c) reinterpret_cast<uint16_t*>(d)[c] = s[c];
         }
-        if (p.zero) {
+        if constexpr (kZero) {
           for (int i = lane; i < L::kRows << p.log_zero_vecs; i += 32) {
             const int r = i >> p.log_zero_vecs, v = (i & ((1 << p.log_zero_vecs) - 1)) * 16;
             if (v >= count) continue;
             const uint8_t* z = p.zero + row_at(r) + v;
-            uint8_t* d = base + scale_bytes + r * p.zero_pitch + v;
+            uint8_t* d = base + L::kScaleBytes + r * kW4ZeroPitch + v;
             if (v + 16 <= count && (reinterpret_cast<uintptr_t>(z) & 15) == 0) cp_async16(smem_u32(d), z);
             else
               for (int c = 0; c < min(16, count - v); ++c) d[c] = z[c];
@@ -381,11 +382,11 @@ w4_m_grouped_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
           for (int v = 0; v < 4; ++v) acc[i][j][v] = 0.f;
 
       // blocks [0, valid) of this warp's part of the stage in `slot`; grp0: staged group of the first
-      auto multiply = [&](auto with_zero, auto whole, int grp0, int valid) {
-        constexpr bool kZero = decltype(with_zero)::value, kWhole = decltype(whole)::value;
+      auto multiply = [&](auto whole, int grp0, int valid) {
+        constexpr bool kWhole = decltype(whole)::value;
         const uint8_t* const st = smem + slot * L::kStageBytes;
-        const uint8_t* const s_frag = staged + (use & 1u) * staged_bytes + lr * p.scale_pitch;
-        const uint8_t* const z_frag = staged + (use & 1u) * staged_bytes + scale_bytes + lr * p.zero_pitch;
+        const uint8_t* const s_frag = staged + (use & 1u) * L::kStagedBytes + lr * kW4ScalePitch;
+        const uint8_t* const z_frag = staged + (use & 1u) * L::kStagedBytes + L::kScaleBytes + lr * kW4ZeroPitch;
 #pragma unroll
         for (int b0 = 0; b0 < kBlocks; b0 += kPer) {
           if (!kWhole && b0 >= valid) break;   // k is a multiple of the group: a started run of kPer blocks is whole
@@ -395,7 +396,7 @@ w4_m_grouped_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
           for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int h = 0; h < 2; ++h)
-              zp[i][h] = zero_pair<kFp16>(kZero ? z_frag[(tile_row(i) + h * 8) * p.zero_pitch + grp] : 8u);
+              zp[i][h] = zero_pair<kFp16>(kZero ? z_frag[(tile_row(i) + h * 8) * kW4ZeroPitch + grp] : 8u);
           float part[2][kNT][4];
 #pragma unroll
           for (int b = b0; b < b0 + kPer; ++b) {
@@ -424,9 +425,9 @@ w4_m_grouped_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
           }
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const uint8_t* sa = s_frag + tile_row(i) * p.scale_pitch + grp * 2;
+            const uint8_t* sa = s_frag + tile_row(i) * kW4ScalePitch + grp * 2;
             const float s0 = to_float<kFp16>(*reinterpret_cast<const uint16_t*>(sa));
-            const float s1 = to_float<kFp16>(*reinterpret_cast<const uint16_t*>(sa + 8 * p.scale_pitch));
+            const float s1 = to_float<kFp16>(*reinterpret_cast<const uint16_t*>(sa + 8 * kW4ScalePitch));
 #pragma unroll
             for (int j = 0; j < kNT; ++j) {
               if (kNT > 1 && j >= nt_used) break;
@@ -440,20 +441,14 @@ w4_m_grouped_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
       };
 
       for (int st0 = 0; st0 < stages; st0 += kWindowStages, ++use) {
-        ok = ok && wait_bounded(scale_full_bar(use & 1u), (use >> 1) & 1u, &s_abort, p.status, kDevTimeoutMma);
+        ok = ok && wait_bounded_parked(scale_full_bar(use & 1u), (use >> 1) & 1u, &s_abort, p.status, kDevTimeoutMma);
         const int st_end = min(stages, st0 + kWindowStages);
         for (int st = st0; st < st_end; ++st) {
-          ok = ok && wait_bounded(full_bar(slot), phase, &s_abort, p.status, kDevTimeoutMma);
+          ok = ok && wait_bounded_parked(full_bar(slot), phase, &s_abort, p.status, kDevTimeoutMma);
           if (!ok) continue;
           const int grp0 = ((st - st0) * kSB + wk * kBlocks) >> kLogGs;
-          if ((st + 1) * kSB <= nblk) {
-            if (p.zero) multiply(std::true_type{}, std::true_type{}, grp0, kBlocks);
-            else multiply(std::false_type{}, std::true_type{}, grp0, kBlocks);
-          } else {
-            const int valid = nblk - st * kSB - wk * kBlocks;
-            if (p.zero) multiply(std::true_type{}, std::false_type{}, grp0, valid);
-            else multiply(std::false_type{}, std::false_type{}, grp0, valid);
-          }
+          if ((st + 1) * kSB <= nblk) multiply(std::true_type{}, grp0, kBlocks);
+          else multiply(std::false_type{}, grp0, nblk - st * kSB - wk * kBlocks);
           __syncwarp();
           if (lane == 0) mbar_arrive(empty_bar(slot));
           if (++slot == kStages) {
@@ -581,14 +576,14 @@ struct W4Operands {
   const void* w;
 };
 
-template <int kWN, int kWK, int kNT, int kStages, int kSB, int kLogGs, bool kGated, bool kFp16>
+template <int kWN, int kWK, int kNT, int kStages, int kSB, int kLogGs, bool kGated, bool kFp16, bool kZero>
 static int launch_w4(const W4Operands& o, W4Args p, int want_sms, cudaStream_t stream) {
   using L = W4Smem<kWN, kWK, kNT, kStages, kSB>;
   static_assert((kW4WindowGroups << kLogGs) % kSB == 0, "a window ends with a stage");
-  auto kern = w4_m_grouped_kernel<kWN, kWK, kNT, kStages, kSB, kLogGs, kGated, kFp16>;
+  auto kern = w4_m_grouped_kernel<kWN, kWK, kNT, kStages, kSB, kLogGs, kGated, kFp16, kZero>;
   constexpr int kOutCols = kGated ? L::kRows / 2 : L::kRows;
   p.tiles = (p.n + kOutCols - 1) / kOutCols;
-  const int smem = L::kScaleOffset + 2 * L::kRows * (p.scale_pitch + p.zero_pitch) +
+  const int smem = L::kScaleOffset + 2 * L::kStagedBytes +
                    p.list_capacity * static_cast<int>(sizeof(W4Expert)) + 1024;
   CUtensorMap tm_w, tm_a;
   {
@@ -621,7 +616,9 @@ static int launch_w4(const W4Operands& o, W4Args p, int want_sms, cudaStream_t s
 
 template <int kWN, int kWK, int kNT, int kStages, int kSB>
 static int form_w4(const W4Operands& o, const W4Args& p, int log_gs, int gated, int dtype, int want_sms, cudaStream_t stream) {
-#define B200_W4(GS, GATED, FP16) launch_w4<kWN, kWK, kNT, kStages, kSB, GS, GATED, FP16>(o, p, want_sms, stream)
+#define B200_W4(GS, GATED, FP16)                                                                 \
+  (p.zero ? launch_w4<kWN, kWK, kNT, kStages, kSB, GS, GATED, FP16, true>(o, p, want_sms, stream) \
+          : launch_w4<kWN, kWK, kNT, kStages, kSB, GS, GATED, FP16, false>(o, p, want_sms, stream))
 #define B200_W4_GS(GATED, FP16) \
   (log_gs == 0 ? B200_W4(0, GATED, FP16) : log_gs == 1 ? B200_W4(1, GATED, FP16) : B200_W4(2, GATED, FP16))
   return gated ? (dtype ? B200_W4_GS(true, true) : B200_W4_GS(true, false))
@@ -664,8 +661,6 @@ static int w4_m_grouped(const void* a, const void* w4, const void* scale, const 
   p.act = act;
   const int groups = k / group_size;
   const int window = groups < kW4WindowGroups ? groups : kW4WindowGroups;
-  p.scale_pitch = ((window * 2 + 15) / 16 | 1) * 16;
-  p.zero_pitch = zero ? ((window + 15) / 16 | 1) * 16 : 0;
   p.log_scale_vecs = window <= 8 ? 0 : window <= 16 ? 1 : 2;
   p.log_zero_vecs = window <= 16 ? 0 : 1;
   p.list_capacity = static_cast<int>(m_rows < num_groups ? m_rows : num_groups);
