@@ -150,7 +150,7 @@ struct W4Smem {
 };
 
 template <int kWN, int kWK, int kNT, int kStages, int kSB, int kLogGs, bool kGated, bool kFp16, bool kZero>
-__global__ void __launch_bounds__(kWN * kWK * 32 + 64, kNT == 1 ? 2 : 1)
+__global__ void __launch_bounds__(kWN * kWK * 32 + 64, kNT <= 2 ? 2 : 1)
 w4_m_grouped_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_a, const W4Args p) {
   using L = W4Smem<kWN, kWK, kNT, kStages, kSB>;
   constexpr int kBlocks = kSB / kWK;                // 32-wide k blocks of a stage that one warp multiplies
@@ -382,8 +382,9 @@ w4_m_grouped_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
           for (int v = 0; v < 4; ++v) acc[i][j][v] = 0.f;
 
       // blocks [0, valid) of this warp's part of the stage in `slot`; grp0: staged group of the first
-      auto multiply = [&](auto whole, int grp0, int valid) {
+      auto multiply = [&](auto whole, auto columns, int grp0, int valid) {
         constexpr bool kWhole = decltype(whole)::value;
+        constexpr int kJ = decltype(columns)::value;   // 8-row column tiles of `a` in use
         const uint8_t* const st = smem + slot * L::kStageBytes;
         const uint8_t* const s_frag = staged + (use & 1u) * L::kStagedBytes + lr * kW4ScalePitch;
         const uint8_t* const z_frag = staged + (use & 1u) * L::kStagedBytes + L::kScaleBytes + lr * kW4ZeroPitch;
@@ -397,7 +398,7 @@ w4_m_grouped_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
 #pragma unroll
             for (int h = 0; h < 2; ++h)
               zp[i][h] = zero_pair<kFp16>(kZero ? z_frag[(tile_row(i) + h * 8) * kW4ZeroPitch + grp] : 8u);
-          float part[2][kNT][4];
+          float part[2][kJ][4];
 #pragma unroll
           for (int b = b0; b < b0 + kPer; ++b) {
             uint32_t wv[2][2][4];
@@ -408,8 +409,7 @@ w4_m_grouped_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
                 unpack_word<kFp16>(*reinterpret_cast<const uint32_t*>(st + w_off[b] + (tile_row(i) + h * 8) * 128), zp[i][h],
                                    wv[i][h]);
 #pragma unroll
-            for (int j = 0; j < kNT; ++j) {
-              if (kNT > 1 && j >= nt_used) break;
+            for (int j = 0; j < kJ; ++j) {
               const uint4 q = *reinterpret_cast<const uint4*>(st + a_off[b & 1] + (b >> 1) * kNT * 1024 + j * 1024);
               const uint32_t x04 = __byte_perm(q.x, q.z, 0x5410), x15 = __byte_perm(q.x, q.z, 0x7632);
               const uint32_t x26 = __byte_perm(q.y, q.w, 0x5410), x37 = __byte_perm(q.y, q.w, 0x7632);
@@ -429,8 +429,7 @@ w4_m_grouped_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
             const float s0 = to_float<kFp16>(*reinterpret_cast<const uint16_t*>(sa));
             const float s1 = to_float<kFp16>(*reinterpret_cast<const uint16_t*>(sa + 8 * kW4ScalePitch));
 #pragma unroll
-            for (int j = 0; j < kNT; ++j) {
-              if (kNT > 1 && j >= nt_used) break;
+            for (int j = 0; j < kJ; ++j) {
               acc[i][j][0] = fmaf(s0, part[i][j][0], acc[i][j][0]);
               acc[i][j][1] = fmaf(s0, part[i][j][1], acc[i][j][1]);
               acc[i][j][2] = fmaf(s1, part[i][j][2], acc[i][j][2]);
@@ -447,8 +446,15 @@ w4_m_grouped_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
           ok = ok && wait_bounded_parked(full_bar(slot), phase, &s_abort, p.status, kDevTimeoutMma);
           if (!ok) continue;
           const int grp0 = ((st - st0) * kSB + wk * kBlocks) >> kLogGs;
-          if ((st + 1) * kSB <= nblk) multiply(std::true_type{}, grp0, kBlocks);
-          else multiply(std::false_type{}, grp0, nblk - st * kSB - wk * kBlocks);
+          const bool whole = (st + 1) * kSB <= nblk;
+          const int valid = nblk - st * kSB - wk * kBlocks;
+          if (kNT > 1 && nt_used == 1) {
+            if (whole) multiply(std::true_type{}, std::integral_constant<int, 1>{}, grp0, kBlocks);
+            else multiply(std::false_type{}, std::integral_constant<int, 1>{}, grp0, valid);
+          } else {
+            if (whole) multiply(std::true_type{}, std::integral_constant<int, kNT>{}, grp0, kBlocks);
+            else multiply(std::false_type{}, std::integral_constant<int, kNT>{}, grp0, valid);
+          }
           __syncwarp();
           if (lane == 0) mbar_arrive(empty_bar(slot));
           if (++slot == kStages) {
@@ -603,7 +609,7 @@ static int launch_w4(const W4Operands& o, W4Args p, int want_sms, cudaStream_t s
       return rc;
   }
   B200_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  const int per_sm = kNT == 1 && 2 * (smem + 2048) <= 228 * 1024 ? 2 : 1;
+  const int per_sm = kNT <= 2 && 2 * (smem + 2048) <= 228 * 1024 ? 2 : 1;
   // at most this many items: every expert with rows has one partial chunk at most
   const long long chunks = p.m_rows / (kNT * 8) + (p.m_rows < p.num_groups ? p.m_rows : p.num_groups);
   const long long items = chunks * p.tiles;
@@ -669,7 +675,7 @@ static int w4_m_grouped(const void* a, const void* w4, const void* scale, const 
   const int log_gs = group_size == 32 ? 0 : group_size == 64 ? 1 : 2;
   const W4Operands o = {a, w4};
   return m_rows <= 8ll * num_groups ? form_w4<2, 4, 1, 3, 16>(o, p, log_gs, gated, dtype, want, stream)
-                                    : form_w4<4, 2, 4, 4, 8>(o, p, log_gs, gated, dtype, want, stream);
+                                    : form_w4<2, 4, 2, 4, 8>(o, p, log_gs, gated, dtype, want, stream);
 }
 
 static int w4_quant(const void* w, void* q, void* scale, void* zero, int64_t rows, int k, int group_size, int dtype,
