@@ -6,6 +6,7 @@ raised -- nothing in this package computes on the CPU or through another GEMM li
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import threading
 from ctypes import c_char_p, c_int, c_int64, c_void_p, c_uint, POINTER, c_float
@@ -151,7 +152,16 @@ def require_cuda(*tensors: torch.Tensor) -> None:
 
 
 def stream_ptr(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    # the raw handle, without a Stream object around it (2.2 us of a call)
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if device.index is None else device.index)
+
+
+_no_guard = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """``with on_device(t.device):`` - a device guard that costs nothing where that device is current already."""
+    return _no_guard if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def ptr(t: torch.Tensor) -> int:

@@ -150,7 +150,7 @@ struct W4Smem {
 };
 
 template <int kWN, int kWK, int kNT, int kStages, int kSB, int kLogGs, bool kGated, bool kFp16, bool kZero>
-__global__ void __launch_bounds__(kWN * kWK * 32 + 64, kNT <= 2 ? 2 : 1)
+__global__ void __launch_bounds__(kWN * kWK * 32 + 64, kNT > 1 || kWN > 1 ? 2 : 3)
 w4_m_grouped_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_a, const W4Args p) {
   using L = W4Smem<kWN, kWK, kNT, kStages, kSB>;
   constexpr int kBlocks = kSB / kWK;                // 32-wide k blocks of a stage that one warp multiplies
@@ -190,61 +190,72 @@ w4_m_grouped_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
     prefetch_tmap(&tm_a);
   }
 
-  // ---- the experts that have rows, in order, by one warp: lane i looks at expert 32 c + i
+  // ---- the experts that have rows, in order, by one warp: lane i looks at experts 128 c + 4 i .. + 3
   if (warp == 0) {
     long long row = 0;   // rows before this chunk of experts
     int active = 0, items = 0;
     bool overflow = false;
-    constexpr int kAhead = 4;   // chunks whose sizes are on their way together
-    long long ahead[kAhead];
-    for (int g0 = 0; g0 < p.num_groups; g0 += 32) {
-      const int which = (g0 >> 5) & (kAhead - 1);
-      if (which == 0) {
+    for (int g0 = 0; g0 < p.num_groups; g0 += 128) {
+      long long end[4];    // after each of the lane's experts, counted from the lane's first
+      long long sum = 0;
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-          const int g = g0 + i * 32 + lane;
-          ahead[i] = 0;
-          if (g < p.num_groups)
-            ahead[i] = p.sizes_i64 ? static_cast<const long long*>(p.sizes)[g]
-                                   : static_cast<long long>(static_cast<const int*>(p.sizes)[g]);
+      for (int i = 0; i < 4; ++i) {
+        const int g = g0 + lane * 4 + i;
+        long long v = 0;
+        if (g < p.num_groups)
+          v = p.sizes_i64 ? static_cast<const long long*>(p.sizes)[g]
+                          : static_cast<long long>(static_cast<const int*>(p.sizes)[g]);
+        end[i] = v;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (end[i] < 0) end[i] = 0;
+        if (end[i] > p.m_rows) {   // cut off below, like every M-grouped entry point; keeps the sums in range
+          end[i] = p.m_rows;
+          overflow = true;
+        }
+        end[i] = sum += end[i];
+      }
+      long long before = sum;      // becomes the rows up to and including this lane's experts
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long up = __shfl_up_sync(0xFFFFFFFFu, before, o);
+        if (lane >= o) before += up;
+      }
+      before += row - sum;
+      int begin[4], rows[4], work[4], mine_active = 0, mine_items = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const long long lo = before + (i ? end[i - 1] : 0), hi = before + end[i];
+        overflow |= hi > p.m_rows && hi > lo;
+        begin[i] = static_cast<int>(lo < p.m_rows ? lo : p.m_rows);
+        rows[i] = static_cast<int>(hi < p.m_rows ? hi : p.m_rows) - begin[i];
+        work[i] = (rows[i] + kNT * 8 - 1) / (kNT * 8) * p.tiles;
+        mine_active += rows[i] > 0;
+        mine_items += work[i];
+      }
+      row = __shfl_sync(0xFFFFFFFFu, before + sum, 31);
+      if (row > p.m_rows) row = p.m_rows;
+      int upto_active = mine_active, upto_items = mine_items;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int a = __shfl_up_sync(0xFFFFFFFFu, upto_active, o), b = __shfl_up_sync(0xFFFFFFFFu, upto_items, o);
+        if (lane >= o) {
+          upto_active += a;
+          upto_items += b;
         }
       }
-      const int g = g0 + lane;
-      long long v = which == 0 ? ahead[0] : which == 1 ? ahead[1] : which == 2 ? ahead[2] : ahead[3];
-      if (v < 0) v = 0;
-      if (v > p.m_rows) {   // cut off below, like every M-grouped entry point; keeps the sums in range
-        v = p.m_rows;
-        overflow = true;
-      }
-      long long end = v;
+      int at = active + upto_active - mine_active, item0 = items + upto_items - mine_items;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long up = __shfl_up_sync(0xFFFFFFFFu, end, o);
-        if (lane >= o) end += up;
+      for (int i = 0; i < 4; ++i) {
+        if (rows[i] > 0) {
+          if (at < p.list_capacity) list[at] = {g0 + lane * 4 + i, begin[i], rows[i], item0};
+          ++at;
+          item0 += work[i];
+        }
       }
-      end += row;
-      long long begin = end - v;
-      if (end > p.m_rows) {
-        overflow |= v > 0;
-        end = p.m_rows;
-        if (begin > p.m_rows) begin = p.m_rows;
-      }
-      row = __shfl_sync(0xFFFFFFFFu, end, 31);
-      const int rows = static_cast<int>(end - begin);
-      const unsigned has = __ballot_sync(0xFFFFFFFFu, rows > 0);
-      const int mine = rows > 0 ? (rows + kNT * 8 - 1) / (kNT * 8) * p.tiles : 0;
-      int upto = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int up = __shfl_up_sync(0xFFFFFFFFu, upto, o);
-        if (lane >= o) upto += up;
-      }
-      if (rows > 0) {
-        const int at = active + __popc(has & ((1u << lane) - 1));
-        if (at < p.list_capacity) list[at] = {g, static_cast<int>(begin), rows, items + upto - mine};
-      }
-      active += __popc(has);
-      items += __shfl_sync(0xFFFFFFFFu, upto, 31);
+      active += __shfl_sync(0xFFFFFFFFu, upto_active, 31);
+      items += __shfl_sync(0xFFFFFFFFu, upto_items, 31);
     }
     if (lane == 0) {
       s_active = active < p.list_capacity ? active : p.list_capacity;
@@ -609,7 +620,8 @@ static int launch_w4(const W4Operands& o, W4Args p, int want_sms, cudaStream_t s
       return rc;
   }
   B200_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  const int per_sm = kNT <= 2 && 2 * (smem + 2048) <= 228 * 1024 ? 2 : 1;
+  // what the registers (see __launch_bounds__) and the shared memory allow
+  const int per_sm = min(kNT > 1 || kWN > 1 ? 2 : 3, 228 * 1024 / (smem + 2048));
   // at most this many items: every expert with rows has one partial chunk at most
   const long long chunks = p.m_rows / (kNT * 8) + (p.m_rows < p.num_groups ? p.m_rows : p.num_groups);
   const long long items = chunks * p.tiles;
@@ -674,6 +686,9 @@ static int w4_m_grouped(const void* a, const void* w4, const void* scale, const 
   const int want = num_sms > 0 && num_sms < sms ? num_sms : sms;
   const int log_gs = group_size == 32 ? 0 : group_size == 64 ? 1 : 2;
   const W4Operands o = {a, w4};
+  const long long rows_at_most = m_rows < num_groups ? m_rows : num_groups;
+  if (m_rows <= 8ll * num_groups && rows_at_most * ((gated ? 2ll * n : n) / 64) <= 2ll * want)
+    return form_w4<1, 8, 1, 3, 16>(o, p, log_gs, gated, dtype, want, stream);
   return m_rows <= 8ll * num_groups ? form_w4<2, 4, 1, 3, 16>(o, p, log_gs, gated, dtype, want, stream)
                                     : form_w4<2, 4, 2, 4, 8>(o, p, log_gs, gated, dtype, want, stream);
 }

@@ -29,7 +29,7 @@ def _check_plan(what: str, pos: torch.Tensor, order: torch.Tensor, pairs: int, d
 def _permute(x, pos, order, top_k):
     t, h = x.shape
     out = x.new_empty(order.numel(), h)
-    with torch.cuda.device(x.device):
+    with _lib.on_device(x.device):
         rc = _lib.load().b200moe_permute_rows(x.data_ptr(), pos.data_ptr(), order.data_ptr(), out.data_ptr(), t, top_k, h,
                                               order.numel(), _lib.stream_ptr(x.device))
     _lib.check(rc, "b200moe_permute_rows")
@@ -39,7 +39,7 @@ def _permute(x, pos, order, top_k):
 def _combine(rows, w32, pos, order, tokens, top_k):
     r, h = rows.shape
     out = rows.new_empty(tokens, h)
-    with torch.cuda.device(rows.device):
+    with _lib.on_device(rows.device):
         rc = _lib.load().b200moe_combine_rows(rows.data_ptr(), pos.data_ptr(), order.data_ptr(),
                                               w32.data_ptr() if w32 is not None else None, out.data_ptr(), tokens, top_k, h, r,
                                               _lib.dtype_code(rows.dtype), _lib.stream_ptr(rows.device))
@@ -78,7 +78,7 @@ class _CombineRows(torch.autograd.Function):
         t, h = dout.shape
         drows = dout.new_empty(ctx.num_rows, h) if ctx.needs_input_grad[0] else None
         dw = torch.empty_like(w32) if ctx.needs_input_grad[1] else None
-        with torch.cuda.device(dout.device):
+        with _lib.on_device(dout.device):
             rc = _lib.load().b200moe_combine_rows_grad(
                 dout.data_ptr(), rows.data_ptr() if rows is not None else None, pos.data_ptr(), order.data_ptr(),
                 w32.data_ptr(), drows.data_ptr() if drows is not None else None, dw.data_ptr() if dw is not None else None,

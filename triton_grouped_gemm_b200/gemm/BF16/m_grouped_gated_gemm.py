@@ -62,7 +62,7 @@ def _m_grouped_gated_launch(A: Tensor, B: Tensor, size_per_group: Tensor, activa
         saved = A.new_empty(m, 2 * inter, dtype=torch.int16)
         exps = A.new_empty(lib.b200gemm_gated_exponent_bytes(m, inter), dtype=torch.uint8)
     sizes, is64 = _lib.sizes_arg(size_per_group)
-    with torch.cuda.device(A.device):
+    with _lib.on_device(A.device):
         rc = lib.b200gemm_m_grouped_gated(
             _lib.ptr(A), _lib.ptr(B), _lib.ptr(h), _lib.ptr(saved) if save else None, _lib.ptr(exps) if save else None,
             _lib.ptr(sizes), is64, g, m, int(masked_stride), inter, k, act, code,
@@ -82,7 +82,7 @@ def _m_grouped_gated_grad_launch(dY: Tensor, W2: Tensor, saved: Tensor, exps: Te
     assert dY.dtype == W2.dtype and size_per_group.numel() == g
     dgu = dY.new_empty(m, 2 * inter)
     sizes, is64 = _lib.sizes_arg(size_per_group)
-    with torch.cuda.device(dY.device):
+    with _lib.on_device(dY.device):
         rc = _lib.load().b200gemm_m_grouped_gated_grad(
             _lib.ptr(dY), _lib.ptr(W2), _lib.ptr(saved), _lib.ptr(exps), _lib.ptr(dgu), _lib.ptr(sizes), is64, g, m, inter, k,
             activation_code(activation), _lib.dtype_code(dY.dtype), _lib.ptr(tail) if tail is not None else None,

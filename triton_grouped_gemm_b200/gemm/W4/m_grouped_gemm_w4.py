@@ -53,7 +53,7 @@ def _launch(a: Tensor, b: W4Weight, size_per_group: Tensor, gated: bool, act: in
         assert out.shape == (m, n) and out.dtype == a.dtype and out.is_contiguous() and out.device == a.device, \
             "out should be contiguous, of a's type and device and of shape [M, N]"
     sizes, is64 = _lib.sizes_arg(size_per_group)
-    with torch.cuda.device(a.device):
+    with _lib.on_device(a.device):
         rc = _lib.load().b200gemm_w4_m_grouped(
             _lib.ptr(a), _lib.ptr(w4), _lib.ptr(scale), _lib.ptr(zero) if zero is not None else None, _lib.ptr(out),
             _lib.ptr(sizes), is64, g, m, n, k, group_size, 1 if gated else 0, act, code, int(num_sms),

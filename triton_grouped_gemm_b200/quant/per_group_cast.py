@@ -23,7 +23,7 @@ def per_group_cast_to_w4(w: torch.Tensor, group_size: int = 128, symmetric: bool
     q = w.new_empty(lead + (k // 2,), dtype=torch.uint8)
     scale = w.new_empty(lead + (k // group_size,))
     zero = None if symmetric else w.new_empty(lead + (k // group_size,), dtype=torch.uint8)
-    with torch.cuda.device(w.device):
+    with _lib.on_device(w.device):
         rc = _lib.load().b200quant_w4_group(_lib.ptr(w), _lib.ptr(q), _lib.ptr(scale),
                                             _lib.ptr(zero) if zero is not None else None, lead.numel(), k, group_size, code,
                                             _lib.stream_ptr(w.device))
