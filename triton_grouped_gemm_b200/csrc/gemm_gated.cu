@@ -135,6 +135,7 @@ struct GatedArgs {
   long long m_rows;
   int inter;          // I
   int k;
+  int a_box;          // rows of a TMA box of A: 128, or 32 where groups are short (see a_box_rows)
   int in_fmt;         // UMMA operand format: 0 = f16, 1 = bf16
   int act;
   uint16_t* h;        // forward: [m_rows, I]
@@ -225,6 +226,8 @@ gated_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ C
       if (!w.seek(mt)) break;
       const int row0 = static_cast<int>(w.tile_row0(mt)) + static_cast<int>(rank) * 128;
       const int g = w.g;
+      // only the boxes that hold rows of the group; the others' lanes multiply what lies there and are not stored
+      const int a_boxes = (min(128, static_cast<int>(w.group_row_end()) - row0) + p.a_box - 1) / p.a_box;
       for (int kb = 0; kb < num_kb; ++kb) {
         if (!wait_bounded(empty_bar(stage), phase ^ 1u, abort_flag, p.status, kDevTimeoutProducer)) {
           ok = false;
@@ -247,8 +250,9 @@ gated_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ C
                                  nt * kOutCols + static_cast<int>(rank) * 128 + j * 64, kb * kBlockK, g);
             }
           } else {
-            mbar_arrive_expect_tx(full_bar(stage), L::kStageBytes);
-            tma_load_2d(a_dst, &tm_a, full_bar(stage), kb * kBlockK, row0);
+            mbar_arrive_expect_tx(full_bar(stage), a_boxes * p.a_box * 128 + L::kBBytes);
+            for (int i = 0; i < a_boxes; ++i)
+              tma_load_2d(a_dst + i * p.a_box * 128, &tm_a, full_bar(stage), kb * kBlockK, row0 + i * p.a_box);
             if constexpr (!kBwd) {
               tma_load_4d(b_dst, &tm_b, full_bar(stage), kb * kBlockK, nt * kHalf, 0, g);
               tma_load_4d(b_dst + kHalf * 128, &tm_b, full_bar(stage), kb * kBlockK, nt * kHalf, 1, g);
@@ -688,8 +692,9 @@ static int gated_forward(const void* a, const void* w13, void* h, void* gu, void
   int half;
   gated_form(m_rows, num_groups, masked_stride, inter, 128, ctas, &pair, &half);
   const CUtensorMapDataType dt = dtype == 1 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const int a_box = a_box_rows(m_rows, num_groups, pair);
   GatedMaps t = {};
-  if (int rc = rows_map(&t.a, dt, a, m_rows, k, 128, "A")) return rc;
+  if (int rc = rows_map(&t.a, dt, a, m_rows, k, a_box, "A")) return rc;
   {
     const uint64_t ku = static_cast<uint64_t>(k), iu = static_cast<uint64_t>(inter);
     const uint64_t dims[4] = {ku, iu, 2, static_cast<uint64_t>(num_groups)};
@@ -708,6 +713,7 @@ static int gated_forward(const void* a, const void* w13, void* h, void* gu, void
   p.m_rows = m_rows;
   p.inter = inter;
   p.k = k;
+  p.a_box = a_box;
   p.in_fmt = dtype == 1 ? 0 : 1;
   p.act = act;
   p.h = static_cast<uint16_t*>(h);
@@ -744,8 +750,9 @@ static int gated_backward(const void* dy, const void* w2, const void* gu, const 
   int half;
   gated_form(m_rows, num_groups, 0, inter, 256, ctas, &pair, &half);
   const CUtensorMapDataType dt = dtype == 1 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const int a_box = a_box_rows(m_rows, num_groups, pair);
   GatedMaps t = {};
-  if (int rc = rows_map(&t.a, dt, dy, m_rows, k, 128, "dY")) return rc;
+  if (int rc = rows_map(&t.a, dt, dy, m_rows, k, a_box, "dY")) return rc;
   {
     const uint64_t ku = static_cast<uint64_t>(k), iu = static_cast<uint64_t>(inter);
     const uint64_t dims[3] = {iu, ku, static_cast<uint64_t>(num_groups)};
@@ -762,6 +769,7 @@ static int gated_backward(const void* dy, const void* w2, const void* gu, const 
   p.m_rows = m_rows;
   p.inter = inter;
   p.k = k;
+  p.a_box = a_box;
   p.in_fmt = dtype == 1 ? 0 : 1;
   p.act = act;
   p.exps = const_cast<uint8_t*>(static_cast<const uint8_t*>(exps));
