@@ -222,4 +222,111 @@ struct GroupWalker {
   }
 };
 
+// The same walk for a whole warp, 32 groups at a time: lane i holds group 32 c + i, the prefix sums over the 32 come
+// from two scans, and a tile's group is found with one vote instead of a step (with its dependent load) per group.
+// A call with many short or empty groups spends its time in those steps: 256 groups, 40 of them with rows, K 2048,
+// 768 + 768 columns: 83 us with GroupWalker, 58 us with this.  Every call is made by all 32 lanes.
+struct WarpGroupWalker {
+  const void* sizes;
+  int sizes_i64;
+  int num_groups;
+  int stride;            // as in GroupWalker
+  int tile_rows;
+  int chunk;             // first group of the 32 in the lanes
+  int my_size, my_tile_begin, my_tile_end;
+  long long my_row_begin;
+  int next_tile;         // first tile after the 32
+  long long next_row;    // first row after the 32
+  int g, tile_begin, size;
+  bool overflow;
+  long long row_begin, row_limit;
+
+  __device__ __forceinline__ void load(int first) {
+    const int lane = static_cast<int>(lane_id());
+    const int i = first + lane;
+    chunk = first;
+    long long v = 0;
+    if (i < num_groups)
+      v = sizes_i64 ? static_cast<const long long*>(sizes)[i] : static_cast<long long>(static_cast<const int*>(sizes)[i]);
+    if (v < 0) v = 0;
+    bool over = false;
+    if (stride > 0) {
+      if (v > stride) v = stride;
+    } else if (v > row_limit) {   // cut off below; keeps the sums in range
+      v = row_limit;
+      over = true;
+    }
+    const long long takes = stride < 0 ? (v + 127) / 128 * 128 : v;   // rows up to the next group's
+    long long upto = takes;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long up = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+      if (lane >= o) upto += up;
+    }
+    my_row_begin = next_row + upto - takes;
+    if (stride <= 0) {
+      const long long room = row_limit > my_row_begin ? row_limit - my_row_begin : 0;
+      if (v > room) {
+        v = room;
+        over = true;
+      }
+    }
+    my_size = static_cast<int>(v);
+    const int tiles = (my_size + tile_rows - 1) / tile_rows;
+    int end = tiles;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xFFFFFFFFu, end, o);
+      if (lane >= o) end += up;
+    }
+    my_tile_end = next_tile + end;
+    my_tile_begin = my_tile_end - tiles;
+    overflow |= __any_sync(0xFFFFFFFFu, over) != 0;
+    next_row += __shfl_sync(0xFFFFFFFFu, upto, 31);
+    if (stride <= 0 && next_row > row_limit) next_row = row_limit;
+    next_tile += __shfl_sync(0xFFFFFFFFu, end, 31);
+  }
+
+  __device__ __forceinline__ void init(const void* sizes_, int sizes_i64_, int num_groups_, int stride_, int tile_rows_,
+                                       long long row_limit_) {
+    sizes = sizes_;
+    sizes_i64 = sizes_i64_;
+    num_groups = num_groups_;
+    stride = stride_;
+    tile_rows = tile_rows_;
+    row_limit = row_limit_;
+    overflow = false;
+    next_tile = 0;
+    next_row = 0;
+    load(0);
+  }
+
+  // Move to padded row tile `t` (t must not decrease between calls).  false = past the end; row_begin is then the
+  // number of rows that belong to a group (layouts other than the masked one).
+  __device__ __forceinline__ bool seek(int t) {
+    while (t >= next_tile) {
+      if (chunk + 32 >= num_groups) {
+        row_begin = next_row;
+        return false;
+      }
+      load(chunk + 32);
+    }
+    const int src = __ffs(__ballot_sync(0xFFFFFFFFu, my_tile_end > t)) - 1;
+    g = chunk + src;
+    size = __shfl_sync(0xFFFFFFFFu, my_size, src);
+    tile_begin = __shfl_sync(0xFFFFFFFFu, my_tile_begin, src);
+    row_begin = __shfl_sync(0xFFFFFFFFu, my_row_begin, src);
+    return true;
+  }
+
+  __device__ __forceinline__ long long tile_row0(int t) const {
+    const long long base = stride > 0 ? static_cast<long long>(g) * stride : row_begin;
+    return base + static_cast<long long>(t - tile_begin) * tile_rows;
+  }
+  __device__ __forceinline__ long long group_row_end() const {
+    const long long base = stride > 0 ? static_cast<long long>(g) * stride : row_begin;
+    return base + size;
+  }
+};
+
 }  // namespace b200

@@ -215,7 +215,7 @@ gated_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ C
 
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
-    GroupWalker w;
+    WarpGroupWalker w;
     w.init(p.sizes, p.sizes_i64, p.num_groups, p.masked_stride, kTileRows, p.m_rows);
     int stage = 0;
     uint32_t phase = 0;
@@ -273,7 +273,7 @@ gated_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ C
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer (pair: leader CTA only)
     if (rank == 0) {
-      GroupWalker w;
+      WarpGroupWalker w;
       w.init(p.sizes, p.sizes_i64, p.num_groups, p.masked_stride, kTileRows, p.m_rows);
       const uint32_t fmt = static_cast<uint32_t>(p.in_fmt);
       const uint32_t idesc = make_instr_desc(fmt, fmt, 0u, kBwd ? 1u : 0u, kTileRows, kCols);
@@ -324,7 +324,7 @@ gated_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ C
     }
   } else {
     // ------------------------------------------------------------ epilogue (warps 2..5)
-    GroupWalker w;
+    WarpGroupWalker w;
     w.init(p.sizes, p.sizes_i64, p.num_groups, p.masked_stride, kTileRows, p.m_rows);
     const int quarter = warp & 3;
     uint8_t* epi = smem + L::kEpiOffset + quarter * (L::kEpiBuffers * 4096);

@@ -95,7 +95,7 @@ m_grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_con
 
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer (both CTAs)
-    GroupWalker w;
+    WarpGroupWalker w;
     w.init(sizes, sizes_i64, num_groups, masked_stride, kPairTileM, m_rows);
     int stage = 0;
     uint32_t phase = 0;
@@ -140,7 +140,7 @@ m_grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_con
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer (leader CTA only)
     if (rank == 0) {
-      GroupWalker w;
+      WarpGroupWalker w;
       w.init(sizes, sizes_i64, num_groups, masked_stride, kPairTileM, m_rows);
       const uint32_t a_fmt = kFp8 ? static_cast<uint32_t>(in_fmt & 0xF) : static_cast<uint32_t>(in_fmt);
       const uint32_t b_fmt = kFp8 ? static_cast<uint32_t>((in_fmt >> 4) & 0xF) : static_cast<uint32_t>(in_fmt);
@@ -188,7 +188,7 @@ m_grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_con
     }
   } else {
     // ------------------------------------------------------------ epilogue (warps 2..5, both CTAs)
-    GroupWalker w;
+    WarpGroupWalker w;
     w.init(sizes, sizes_i64, num_groups, masked_stride, kPairTileM, m_rows);
     const int quarter = warp & 3;
     uint8_t* epi_stage = smem + L::kEpiOffset + quarter * kEpiStageBytesPerWarp;
