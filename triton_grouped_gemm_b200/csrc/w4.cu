@@ -50,9 +50,12 @@ struct W4Args {
   long long m_rows;
   int n, k;
   int act;
+  int a_boxes;           // TMA boxes of `a` per stage: 1 where k is a multiple of 64, else one per 64 k
   int tiles;             // tiles per expert
-  int log_scale_vecs;    // log2 of the 16-byte pieces (rounded up to a power of two) of a row's staged scales / zeros
-  int log_zero_vecs;
+  int log_scale_piece;   // log2 bytes of the pieces that scales / zeros are copied in: 16 where every row's begin is
+  int log_zero_piece;    // aligned to that, down to one element
+  int log_scale_pieces;  // log2 of the pieces per staged row, rounded up to a power of two
+  int log_zero_pieces;
   int list_capacity;     // entries of the list of experts with rows
   unsigned* status;
 };
@@ -63,6 +66,16 @@ struct W4Expert {
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async8(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+// this thread's arrival on `bar` once its copies so far have landed
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
@@ -269,33 +282,39 @@ w4_m_grouped_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
   struct Item {
     int g, row0, rows, n0;
   };
-  auto item_at = [&](int item) {
-    int lo = 0, hi = active - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (list[mid].item0 <= item) lo = mid;
-      else hi = mid - 1;
+  // Item by item, in rising order and by a whole warp: `at` is the list entry of the last one, and a vote finds how many
+  // entries further the next one's is.
+  auto item_at = [&](int item, int& at) {
+    for (;;) {
+      const int i = at + 1 + lane;
+      const int step = __popc(__ballot_sync(0xFFFFFFFFu, i < active && list[i < active ? i : 0].item0 <= item));
+      at += step;
+      if (step < 32) break;
     }
-    const W4Expert e = list[lo];
+    const W4Expert e = list[at];
     const int chunks = (e.rows + kNT * 8 - 1) / (kNT * 8);
-    const int tile = (item - e.item0) / chunks;
-    const int chunk = (item - e.item0) - tile * chunks;
+    int tile = item - e.item0, chunk = 0;
+    if (chunks > 1) {
+      const int q = tile / chunks;
+      chunk = tile - q * chunks;
+      tile = q;
+    }
     return Item{e.g, e.row0 + chunk * kNT * 8, min(kNT * 8, e.rows - chunk * kNT * 8), tile * kOutCols};
   };
+  int at = 0;   // every warp walks the list on its own
 
   if (warp == L::kWarps) {
     // ---- the stages of this block's items, by one thread
-    if (lane == 0) {
-      int slot = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      for (int item = blockIdx.x; ok && item < items; item += gridDim.x) {
-        const Item it = item_at(item);
-        for (int st = 0; st < stages; ++st) {
-          if (!wait_bounded_parked(empty_bar(slot), phase ^ 1u, &s_abort, p.status, kDevTimeoutProducer)) {
-            ok = false;
-            break;
-          }
+    int slot = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int item = blockIdx.x; ok && item < items; item += gridDim.x) {
+      const Item it = item_at(item, at);
+      for (int st = 0; st < stages; ++st) {
+        ok = __all_sync(0xFFFFFFFFu,
+                        wait_bounded_parked(empty_bar(slot), phase ^ 1u, &s_abort, p.status, kDevTimeoutProducer));
+        if (!ok) break;
+        if (lane == 0) {
           const uint32_t bar = full_bar(slot), w_dst = smem_base + slot * L::kStageBytes, a_dst = w_dst + L::kWBytes;
           mbar_arrive_expect_tx(bar, L::kStageBytes);
 #pragma unroll
@@ -305,13 +324,17 @@ w4_m_grouped_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
             tma_load_4d(d, &tm_w, bar, x, it.n0, 0, it.g);
             if constexpr (kGated) tma_load_4d(d + L::kRows * 64, &tm_w, bar, x, it.n0, 1, it.g);
           }
+          if (p.a_boxes == 1) {
+            tma_load_3d(a_dst, &tm_a, bar, 0, it.row0, st * (kSB / 2));
+          } else {
 #pragma unroll
-          for (int i = 0; i < kSB / 2; ++i)
-            tma_load_2d(a_dst + i * kNT * 1024, &tm_a, bar, st * (kSB * 32) + i * 64, it.row0);
-          if (++slot == kStages) {
-            slot = 0;
-            phase ^= 1u;
+            for (int i = 0; i < kSB / 2; ++i)
+              tma_load_2d(a_dst + i * kNT * 1024, &tm_a, bar, st * (kSB * 32) + i * 64, it.row0);
           }
+        }
+        if (++slot == kStages) {
+          slot = 0;
+          phase ^= 1u;
         }
       }
     }
@@ -321,41 +344,47 @@ w4_m_grouped_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
     uint32_t use = 0;
     bool ok = true;
     for (int item = blockIdx.x; ok && item < items; item += gridDim.x) {
-      const Item it = item_at(item);
+      const Item it = item_at(item, at);
+      // first rows of the tile's (gate) rows and of its up rows
+      const long long row_a = (static_cast<long long>(it.g) * weight_rows + it.n0) * groups;
+      const long long row_b = row_a + static_cast<long long>(p.n) * groups;
+      const int last = p.n - 1 - it.n0;
       for (int first = 0; first < groups; first += kW4WindowGroups, ++use) {
         const int buf = use & 1u;
-        if (!wait_bounded_parked(scale_empty_bar(buf), ((use >> 1) & 1u) ^ 1u, &s_abort, p.status, kDevTimeoutProducer)) {
-          ok = false;
-          break;
-        }
+        ok = __all_sync(0xFFFFFFFFu, wait_bounded_parked(scale_empty_bar(buf), ((use >> 1) & 1u) ^ 1u, &s_abort, p.status,
+                                                         kDevTimeoutProducer));
+        if (!ok) break;
         const int count = min(kW4WindowGroups, groups - first);
         uint8_t* const base = staged + buf * L::kStagedBytes;
         auto row_at = [&](int r) {
-          const int col = min(it.n0 + (kGated ? r % kOutCols : r), p.n - 1);
-          return (static_cast<long long>(it.g) * weight_rows + (kGated && r >= kOutCols ? p.n + col : col)) * groups + first;
+          const bool up = kGated && r >= kOutCols;
+          return (up ? row_b : row_a) + first + min(up ? r - kOutCols : r, last) * groups;
         };
-        for (int i = lane; i < L::kRows << p.log_scale_vecs; i += 32) {
-          const int r = i >> p.log_scale_vecs, v = (i & ((1 << p.log_scale_vecs) - 1)) * 8;   // 8 scales
-          if (v >= count) continue;
-          const uint16_t* s = reinterpret_cast<const uint16_t*>(p.scale) + row_at(r) + v;
-          uint8_t* d = base + r * kW4ScalePitch + v * 2;
-          if (v + 8 <= count && (reinterpret_cast<uintptr_t>(s) & 15) == 0) cp_async16(smem_u32(d), s);
-          else
-            for (int c = 0; c < min(8, count - v); ++c) reinterpret_cast<uint16_t*>(d)[c] = s[c];
-        }
-        if constexpr (kZero) {
-          for (int i = lane; i < L::kRows << p.log_zero_vecs; i += 32) {
-            const int r = i >> p.log_zero_vecs, v = (i & ((1 << p.log_zero_vecs) - 1)) * 16;
-            if (v >= count) continue;
-            const uint8_t* z = p.zero + row_at(r) + v;
-            uint8_t* d = base + L::kScaleBytes + r * kW4ZeroPitch + v;
-            if (v + 16 <= count && (reinterpret_cast<uintptr_t>(z) & 15) == 0) cp_async16(smem_u32(d), z);
-            else
-              for (int c = 0; c < min(16, count - v); ++c) d[c] = z[c];
+        // `count` elements of `elem` bytes per row, in pieces of 1 << log_piece bytes, lane after lane
+        auto stage = [&](const uint8_t* src, uint8_t* dst, int pitch, int elem, int log_piece, int log_pieces) {
+          const int bytes = count * elem;
+#pragma unroll 4
+          for (int i = lane; i < L::kRows << log_pieces; i += 32) {
+            const int r = i >> log_pieces, at = (i & ((1 << log_pieces) - 1)) << log_piece;
+            if (at >= bytes) continue;
+            const uint8_t* s = src + row_at(r) * elem + at;
+            uint8_t* d = dst + r * pitch + at;
+            if (log_piece == 4) cp_async16(smem_u32(d), s);
+            else if (log_piece == 3) cp_async8(smem_u32(d), s);
+            else if (log_piece == 2) cp_async4(smem_u32(d), s);
+            else if (log_piece == 1) *reinterpret_cast<uint16_t*>(d) = *reinterpret_cast<const uint16_t*>(s);
+            else *d = *s;
           }
+        };
+        stage(p.scale, base, kW4ScalePitch, 2, p.log_scale_piece, p.log_scale_pieces);
+        if constexpr (kZero) stage(p.zero, base + L::kScaleBytes, kW4ZeroPitch, 1, p.log_zero_piece, p.log_zero_pieces);
+        // every lane arrives for its own pieces; with copies alone the warp goes on to the next item meanwhile
+        if (p.log_scale_piece >= 2 && (!kZero || p.log_zero_piece >= 2)) {
+          cp_async_arrive(scale_full_bar(buf));
+        } else {
+          cp_async_wait_all();
+          mbar_arrive(scale_full_bar(buf));
         }
-        cp_async_wait_all();
-        mbar_arrive(scale_full_bar(buf));   // every lane: its own copies and stores are done
       }
     }
   } else {
@@ -382,7 +411,7 @@ w4_m_grouped_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
     int red_buf = 0;
     bool ok = true;   // false: a wait ran out; the rest is walked through without touching data
     for (int item = blockIdx.x; item < items; item += gridDim.x, red_buf ^= 1) {
-      const Item it = item_at(item);
+      const Item it = item_at(item, at);
       const int nt_used = (it.rows + 7) >> 3;
       float acc[2][kNT][4];
 #pragma unroll
@@ -392,80 +421,86 @@ w4_m_grouped_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
 #pragma unroll
           for (int v = 0; v < 4; ++v) acc[i][j][v] = 0.f;
 
-      // blocks [0, valid) of this warp's part of the stage in `slot`; grp0: staged group of the first
-      auto multiply = [&](auto whole, auto columns, int grp0, int valid) {
-        constexpr bool kWhole = decltype(whole)::value;
+      // `count` blocks of the stage in `slot` that share a scale, staged group `grp`; w_at(b), a_at(b): where block b's
+      // fragments begin
+      auto run = [&](auto columns, auto blocks, int grp, auto&& w_at, auto&& a_at) {
         constexpr int kJ = decltype(columns)::value;   // 8-row column tiles of `a` in use
+        constexpr int kCount = decltype(blocks)::value;
         const uint8_t* const st = smem + slot * L::kStageBytes;
         const uint8_t* const s_frag = staged + (use & 1u) * L::kStagedBytes + lr * kW4ScalePitch;
         const uint8_t* const z_frag = staged + (use & 1u) * L::kStagedBytes + L::kScaleBytes + lr * kW4ZeroPitch;
+        uint32_t zp[2][2];
 #pragma unroll
-        for (int b0 = 0; b0 < kBlocks; b0 += kPer) {
-          if (!kWhole && b0 >= valid) break;   // k is a multiple of the group: a started run of kPer blocks is whole
-          const int grp = grp0 + (b0 >> kLogGs);
-          uint32_t zp[2][2];
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            zp[i][h] = zero_pair<kFp16>(kZero ? z_frag[(tile_row(i) + h * 8) * kW4ZeroPitch + grp] : 8u);
+        float part[2][kJ][4];
+#pragma unroll
+        for (int b = 0; b < kCount; ++b) {
+          const uint8_t* const w_frag = st + w_at(b);
+          const uint8_t* const a_frag = st + a_at(b);
+          uint32_t wv[2][2][4];
 #pragma unroll
           for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int h = 0; h < 2; ++h)
-              zp[i][h] = zero_pair<kFp16>(kZero ? z_frag[(tile_row(i) + h * 8) * kW4ZeroPitch + grp] : 8u);
-          float part[2][kJ][4];
+              unpack_word<kFp16>(*reinterpret_cast<const uint32_t*>(w_frag + (tile_row(i) + h * 8) * 128), zp[i][h], wv[i][h]);
 #pragma unroll
-          for (int b = b0; b < b0 + kPer; ++b) {
-            uint32_t wv[2][2][4];
+          for (int j = 0; j < kJ; ++j) {
+            const uint4 q = *reinterpret_cast<const uint4*>(a_frag + j * 1024);
+            const uint32_t x04 = __byte_perm(q.x, q.z, 0x5410), x15 = __byte_perm(q.x, q.z, 0x7632);
+            const uint32_t x26 = __byte_perm(q.y, q.w, 0x5410), x37 = __byte_perm(q.y, q.w, 0x7632);
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-              for (int h = 0; h < 2; ++h)
-                unpack_word<kFp16>(*reinterpret_cast<const uint32_t*>(st + w_off[b] + (tile_row(i) + h * 8) * 128), zp[i][h],
-                                   wv[i][h]);
-#pragma unroll
-            for (int j = 0; j < kJ; ++j) {
-              const uint4 q = *reinterpret_cast<const uint4*>(st + a_off[b & 1] + (b >> 1) * kNT * 1024 + j * 1024);
-              const uint32_t x04 = __byte_perm(q.x, q.z, 0x5410), x15 = __byte_perm(q.x, q.z, 0x7632);
-              const uint32_t x26 = __byte_perm(q.y, q.w, 0x5410), x37 = __byte_perm(q.y, q.w, 0x7632);
-#pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                const uint32_t f0[4] = {wv[i][0][0], wv[i][1][0], wv[i][0][1], wv[i][1][1]};
-                const uint32_t f1[4] = {wv[i][0][2], wv[i][1][2], wv[i][0][3], wv[i][1][3]};
-                if (b == b0) mma_16816<kFp16, true>(part[i][j], f0, x04, x15);
-                else mma_16816<kFp16, false>(part[i][j], f0, x04, x15);
-                mma_16816<kFp16, false>(part[i][j], f1, x26, x37);
-              }
+            for (int i = 0; i < 2; ++i) {
+              const uint32_t f0[4] = {wv[i][0][0], wv[i][1][0], wv[i][0][1], wv[i][1][1]};
+              const uint32_t f1[4] = {wv[i][0][2], wv[i][1][2], wv[i][0][3], wv[i][1][3]};
+              if (b == 0) mma_16816<kFp16, true>(part[i][j], f0, x04, x15);
+              else mma_16816<kFp16, false>(part[i][j], f0, x04, x15);
+              mma_16816<kFp16, false>(part[i][j], f1, x26, x37);
             }
           }
+        }
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const uint8_t* sa = s_frag + tile_row(i) * kW4ScalePitch + grp * 2;
-            const float s0 = to_float<kFp16>(*reinterpret_cast<const uint16_t*>(sa));
-            const float s1 = to_float<kFp16>(*reinterpret_cast<const uint16_t*>(sa + 8 * kW4ScalePitch));
+        for (int i = 0; i < 2; ++i) {
+          const uint8_t* sa = s_frag + tile_row(i) * kW4ScalePitch + grp * 2;
+          const float s0 = to_float<kFp16>(*reinterpret_cast<const uint16_t*>(sa));
+          const float s1 = to_float<kFp16>(*reinterpret_cast<const uint16_t*>(sa + 8 * kW4ScalePitch));
 #pragma unroll
-            for (int j = 0; j < kJ; ++j) {
-              acc[i][j][0] = fmaf(s0, part[i][j][0], acc[i][j][0]);
-              acc[i][j][1] = fmaf(s0, part[i][j][1], acc[i][j][1]);
-              acc[i][j][2] = fmaf(s1, part[i][j][2], acc[i][j][2]);
-              acc[i][j][3] = fmaf(s1, part[i][j][3], acc[i][j][3]);
-            }
+          for (int j = 0; j < kJ; ++j) {
+            acc[i][j][0] = fmaf(s0, part[i][j][0], acc[i][j][0]);
+            acc[i][j][1] = fmaf(s0, part[i][j][1], acc[i][j][1]);
+            acc[i][j][2] = fmaf(s1, part[i][j][2], acc[i][j][2]);
+            acc[i][j][3] = fmaf(s1, part[i][j][3], acc[i][j][3]);
           }
+        }
+      };
+      // a stage whose first block is block0 of its window of scales and that holds `held` blocks
+      auto multiply = [&](auto columns, int block0, int held) {
+        if (held >= kSB) {   // a warp's kBlocks neighbours, kPer at a time
+          const int grp = (block0 + wk * kBlocks) >> kLogGs;
+#pragma unroll
+          for (int b0 = 0; b0 < kBlocks; b0 += kPer)
+            run(columns, std::integral_constant<int, kPer>{}, grp + (b0 >> kLogGs), [&](int b) { return w_off[b0 + b]; },
+                [&](int b) { return a_off[(b0 + b) & 1] + ((b0 + b) >> 1) * kNT * 1024; });
+        } else {             // the last stage of a k that is no multiple of it: block by block in turn
+#pragma unroll 1
+          for (int c = wk; c < held; c += kWK)
+            run(columns, std::integral_constant<int, 1>{}, (block0 + c) >> kLogGs,
+                [&](int) { return (c >> 3) * (L::kRows * 128) + lr * 128 + (((c & 7) ^ lr) << 4) + lt * 4; },
+                [&](int) { return L::kWBytes + (c >> 1) * kNT * 1024 + a_row * 128 + ((((c & 1) * 4 + lt) ^ a_row) << 4); });
         }
       };
 
       for (int st0 = 0; st0 < stages; st0 += kWindowStages, ++use) {
-        ok = ok && wait_bounded_parked(scale_full_bar(use & 1u), (use >> 1) & 1u, &s_abort, p.status, kDevTimeoutMma);
+        ok = __all_sync(0xFFFFFFFFu, ok && wait_bounded_parked(scale_full_bar(use & 1u), (use >> 1) & 1u, &s_abort, p.status,
+                                                               kDevTimeoutMma));
         const int st_end = min(stages, st0 + kWindowStages);
         for (int st = st0; st < st_end; ++st) {
-          ok = ok && wait_bounded_parked(full_bar(slot), phase, &s_abort, p.status, kDevTimeoutMma);
+          ok = __all_sync(0xFFFFFFFFu, ok && wait_bounded_parked(full_bar(slot), phase, &s_abort, p.status, kDevTimeoutMma));
           if (!ok) continue;
-          const int grp0 = ((st - st0) * kSB + wk * kBlocks) >> kLogGs;
-          const bool whole = (st + 1) * kSB <= nblk;
-          const int valid = nblk - st * kSB - wk * kBlocks;
-          if (kNT > 1 && nt_used == 1) {
-            if (whole) multiply(std::true_type{}, std::integral_constant<int, 1>{}, grp0, kBlocks);
-            else multiply(std::false_type{}, std::integral_constant<int, 1>{}, grp0, valid);
-          } else {
-            if (whole) multiply(std::true_type{}, std::integral_constant<int, kNT>{}, grp0, kBlocks);
-            else multiply(std::false_type{}, std::integral_constant<int, kNT>{}, grp0, valid);
-          }
+          if (kNT > 1 && nt_used == 1) multiply(std::integral_constant<int, 1>{}, (st - st0) * kSB, nblk - st * kSB);
+          else multiply(std::integral_constant<int, kNT>{}, (st - st0) * kSB, nblk - st * kSB);
           __syncwarp();
           if (lane == 0) mbar_arrive(empty_bar(slot));
           if (++slot == kStages) {
@@ -613,10 +648,15 @@ static int launch_w4(const W4Operands& o, W4Args p, int want_sms, cudaStream_t s
       return rc;
   }
   {
-    const uint64_t dims[2] = {static_cast<uint64_t>(p.k), static_cast<uint64_t>(p.m_rows)};
-    const uint64_t strides[1] = {static_cast<uint64_t>(p.k) * 2};
-    const uint32_t box[2] = {64, kNT * 8};
-    if (int rc = encode_tmap(&tm_a, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, o.a, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, "A"))
+    // seen as [k / 64][m_rows][64] a whole stage of `a` is one box; as [m_rows][k] it takes one per 64 k (a small box
+    // costs the TMA unit as much as a large one)
+    const uint64_t k = static_cast<uint64_t>(p.k), rows = static_cast<uint64_t>(p.m_rows);
+    p.a_boxes = p.k % 64 == 0 ? 1 : kSB / 2;
+    const uint64_t dims[3] = {p.a_boxes == 1 ? 64 : k, rows, k / 64};
+    const uint64_t strides[2] = {k * 2, 128};
+    const uint32_t box[3] = {64, kNT * 8, kSB / 2};
+    if (int rc = encode_tmap(&tm_a, CU_TENSOR_MAP_DATA_TYPE_UINT16, p.a_boxes == 1 ? 3 : 2, o.a, dims, strides, box,
+                             CU_TENSOR_MAP_SWIZZLE_128B, "A"))
       return rc;
   }
   B200_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
@@ -679,8 +719,22 @@ static int w4_m_grouped(const void* a, const void* w4, const void* scale, const 
   p.act = act;
   const int groups = k / group_size;
   const int window = groups < kW4WindowGroups ? groups : kW4WindowGroups;
-  p.log_scale_vecs = window <= 8 ? 0 : window <= 16 ? 1 : 2;
-  p.log_zero_vecs = window <= 16 ? 0 : 1;
+  auto log_piece = [](const void* base, int row_bytes, int least) {
+    int log = 4;
+    while (log > least && ((reinterpret_cast<uintptr_t>(base) | static_cast<unsigned>(row_bytes)) & ((1u << log) - 1))) --log;
+    return log;
+  };
+  auto log_pieces = [](int bytes, int piece) {
+    int log = 0;
+    while ((piece << log) < bytes) ++log;
+    return log;
+  };
+  p.log_scale_piece = log_piece(scale, groups * 2, 1);
+  p.log_scale_pieces = log_pieces(window * 2, 1 << p.log_scale_piece);
+  if (zero) {
+    p.log_zero_piece = log_piece(zero, groups, 0);
+    p.log_zero_pieces = log_pieces(window, 1 << p.log_zero_piece);
+  }
   p.list_capacity = static_cast<int>(m_rows < num_groups ? m_rows : num_groups);
   p.status = device_status_ptr();
   const int want = num_sms > 0 && num_sms < sms ? num_sms : sms;
@@ -689,7 +743,7 @@ static int w4_m_grouped(const void* a, const void* w4, const void* scale, const 
   const long long rows_at_most = m_rows < num_groups ? m_rows : num_groups;
   if (m_rows <= 8ll * num_groups && rows_at_most * ((gated ? 2ll * n : n) / 64) <= 2ll * want)
     return form_w4<1, 8, 1, 3, 16>(o, p, log_gs, gated, dtype, want, stream);
-  return m_rows <= 8ll * num_groups ? form_w4<2, 4, 1, 3, 16>(o, p, log_gs, gated, dtype, want, stream)
+  return m_rows <= 8ll * num_groups ? form_w4<4, 2, 1, 3, 8>(o, p, log_gs, gated, dtype, want, stream)
                                     : form_w4<2, 4, 2, 4, 8>(o, p, log_gs, gated, dtype, want, stream);
 }
 
