@@ -19,8 +19,8 @@
 // A block takes a tile of kWN * 32 weight rows of one expert (gated: half gate, half up rows) and up to kNT * 8 rows
 // of `a`.  kWK warps split each stage of kSB * 32 k; their partial sums are joined in a fixed order, so results do not
 // depend on timing.  Blocks are persistent over the (expert with rows, tile, row chunk) items; an expert's row chunks
-// are neighbours, so the second one finds the weights in L2.  Of two further warps one fetches the stages by TMA and
-// one the scales, both running ahead across the items' borders, so a block never drains, and the multiplying warps
+// are neighbours, so the second one finds the weights in L2.  Of four further warps one fetches the stages by TMA and
+// three the scales, all running ahead across the items' borders, so a block never drains, and the multiplying warps
 // meet only to join their sums.  The 128-byte swizzle makes both operands' fragment loads free of bank conflicts (rows of `a` are taken in
 // the order 0 4 1 5 2 6 3 7 for that).  With the loads off the warps' hands the kernel is bound by the logic
 // pipe (masks, shifts, byte permutes: 24 instructions per 32 x 32 values in fp16, 32 in bf16) until HBM takes over.
@@ -148,8 +148,15 @@ __device__ __forceinline__ void unpack_word(uint32_t w, uint32_t zp, uint32_t (&
 
 template <int kWN, int kWK, int kNT, int kStages, int kSB>
 struct W4Smem {
-  static constexpr int kWarps = kWN * kWK;         // that multiply; two more fetch
-  static constexpr int kThreads = (kWarps + 2) * 32;
+  static constexpr int kWarps = kWN * kWK;         // that multiply; one more fetches stages, three fetch scales
+  static constexpr int kScaleWarps = 3;
+  static constexpr int kThreads = (kWarps + 1 + kScaleWarps) * 32;
+  // Registers of the forms with two blocks per SM: a launch of 384 threads has 80 each; the fetching warpgroup hands
+  // some of its share to the two that multiply.  setmaxnreg.inc waits for registers that must exist in the block's own
+  // allocation, so the shares may not add up to more than the launch's.
+  static constexpr bool kRebalance = kWN > 1;
+  static constexpr int kRegs = 80, kRegsFetch = 48, kRegsMultiply = 96;
+  static_assert(kWarps == 8 && kThreads == 384 && 128 * kRegsFetch + 256 * kRegsMultiply <= 384 * kRegs);
   static constexpr int kRows = kWN * 32;
   static constexpr int kScaleBytes = kRows * kW4ScalePitch;
   static constexpr int kStagedBytes = kRows * (kW4ScalePitch + kW4ZeroPitch);
@@ -163,7 +170,7 @@ struct W4Smem {
 };
 
 template <int kWN, int kWK, int kNT, int kStages, int kSB, int kLogGs, bool kGated, bool kFp16, bool kZero>
-__global__ void __launch_bounds__(kWN * kWK * 32 + 64, kNT > 1 || kWN > 1 ? 2 : 3)
+__global__ void __launch_bounds__(kWN * kWK * 32 + 128, kNT > 1 || kWN > 1 ? 2 : 3)
 w4_m_grouped_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_a, const W4Args p) {
   using L = W4Smem<kWN, kWK, kNT, kStages, kSB>;
   constexpr int kBlocks = kSB / kWK;                // 32-wide k blocks of a stage that one warp multiplies
@@ -194,7 +201,7 @@ w4_m_grouped_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
       mbar_init(empty_bar(s), L::kWarps);
     }
     for (int b = 0; b < 2; ++b) {
-      mbar_init(scale_full_bar(b), 32);
+      mbar_init(scale_full_bar(b), 32 * L::kScaleWarps);
       mbar_init(scale_empty_bar(b), L::kWarps);
     }
     s_abort = 0;
@@ -303,6 +310,10 @@ w4_m_grouped_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
   };
   int at = 0;   // every warp walks the list on its own
 
+  if constexpr (L::kRebalance) {
+    if (warp >= L::kWarps) warpgroup_reg_dec<L::kRegsFetch>();
+    else warpgroup_reg_inc<L::kRegsMultiply>();
+  }
   if (warp == L::kWarps) {
     // ---- the stages of this block's items, by one thread
     int slot = 0;
@@ -338,8 +349,8 @@ w4_m_grouped_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
         }
       }
     }
-  } else if (warp == L::kWarps + 1) {
-    // ---- the scales and zeros of this block's items, kW4WindowGroups groups at a time, by one warp.  Tile row r: gated:
+  } else if (warp > L::kWarps) {
+    // ---- the scales and zeros of this block's items, kW4WindowGroups groups at a time, by three warps.  Tile row r: gated:
     // gate rows, then the up rows of the same outputs; rows past the end are read from the last one.
     uint32_t use = 0;
     bool ok = true;
@@ -364,7 +375,7 @@ w4_m_grouped_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
         auto stage = [&](const uint8_t* src, uint8_t* dst, int pitch, int elem, int log_piece, int log_pieces) {
           const int bytes = count * elem;
 #pragma unroll 4
-          for (int i = lane; i < L::kRows << log_pieces; i += 32) {
+          for (int i = tid - (L::kWarps + 1) * 32; i < L::kRows << log_pieces; i += 32 * L::kScaleWarps) {
             const int r = i >> log_pieces, at = (i & ((1 << log_pieces) - 1)) << log_piece;
             if (at >= bytes) continue;
             const uint8_t* s = src + row_at(r) * elem + at;
@@ -658,6 +669,17 @@ static int launch_w4(const W4Operands& o, W4Args p, int want_sms, cudaStream_t s
     if (int rc = encode_tmap(&tm_a, CU_TENSOR_MAP_DATA_TYPE_UINT16, p.a_boxes == 1 ? 3 : 2, o.a, dims, strides, box,
                              CU_TENSOR_MAP_SWIZZLE_128B, "A"))
       return rc;
+  }
+  if constexpr (L::kRebalance) {   // the build must have given the launch the registers that the split counts on
+    static int launch_regs = 0;
+    if (!launch_regs) {
+      cudaFuncAttributes attr;
+      B200_CUDA(cudaFuncGetAttributes(&attr, kern));
+      launch_regs = attr.numRegs;
+    }
+    if (launch_regs < L::kRegs)
+      return set_error(kErrUnsupported, "b200gemm_w4_m_grouped: built with %d registers per thread, %d are needed", launch_regs,
+                       L::kRegs);
   }
   B200_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   // what the registers (see __launch_bounds__) and the shared memory allow
