@@ -10,11 +10,11 @@
 //     half, side by side in one accumulator.  In the CTA-pair form (256 rows on two SMs) CTA 0 supplies the gate
 //     box and CTA 1 the up box.  No interleaved copy of the weights is needed.
 //   * For training the forward keeps g and u, which the backward epilogue reads back tile by tile into the buffers
-//     it then overwrites with dg and du.  They are kept in 16 bits: a 4-bit exponent and 11-bit mantissa (fp16
-//     layers: 3 and 12) below the largest exponent of 32 neighbouring columns of the row.  That block is what a
-//     thread holds in registers, so its maximum costs no exchange, and the value kept is 16 (fp16: 4) times closer
-//     than bf16 (fp16) would be: what the gradients lose is the rounding of dg and du alone, which the tensor
-//     cores ask for.  Measured on G=16, 4096 rows: error of dx 2.9e-3 with bf16, 2.4e-3 with this.
+//     it then overwrites with dg and du.  They are kept in 16 bits scaled by the largest of 32 neighbouring columns of
+//     the row (see below).  That block is what a thread holds in registers, so its maximum costs no exchange, and what
+//     the gradients lose is the rounding of dg and du alone, which the tensor cores ask for: error of dx in 2-norm,
+//     4096 rows, K 2048, I 768: bf16 layers 2.4e-3, and 3.0e-3 with g and u in bf16 (1.7e-3 is the rounding of dx
+//     itself); fp16 layers 2.9e-4 and 3.8e-4 (2.1e-4).
 //   * Everything else is the M-grouped kernel's: persistent CTAs, one walk over the group sizes, TMA ring, one MMA
 //     issuer, two accumulators, epilogue warps that store through swizzled staging buffers.
 //
@@ -621,16 +621,20 @@ static int halves_map(CUtensorMap* out, CUtensorMapDataType dt, const void* base
   return encode_tmap(out, dt, 3, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, what);
 }
 
-// Which form runs, by the rule of the plain M-grouped kernel: CTA pairs when groups average four 256-row tiles and
-// every pair gets one; else 128-row tiles, `half` = 128 columns of each half wide unless that leaves SMs idle.
-static void gated_form(int64_t m_rows, int num_groups, int masked_stride, int inter, int out_cols_wide, int sms,
-                       bool* pair, int* half) {
+// Which form runs.  CTA pairs when groups average `pair_tiles` 256-row tiles and every pair of SMs gets one; else 128-row
+// tiles, `half` = 128 columns of each half wide unless that leaves SMs idle.  The pair form wastes more of a group's
+// last tile but keeps more of its ring beside the larger staging buffers: with 128 groups, K 2048, 768 + 768 columns
+// the plain forward is even at 1024 rows per group (818 us single, 789 pair), the saving forward and the gradient at
+// 256 (333 against 322 us, 198 against 188) and the gradient 7 % faster at 1024.
+static void gated_form(int64_t m_rows, int num_groups, int masked_stride, int inter, int out_cols_wide, int pair_tiles,
+                       int sms, bool* pair, int* half) {
   const long long tiles_wide = (inter + out_cols_wide - 1) / out_cols_wide;
   *pair = false;
   if (sms >= 2 && masked_stride <= 0) {
     if (g_cta_pair_mode == 1) *pair = true;
     else if (g_cta_pair_mode != 0)
-      *pair = m_rows / 256 * tiles_wide >= sms / 2 && m_rows / 256 >= 4ll * num_groups && inter > out_cols_wide / 2;
+      *pair = m_rows / 256 * tiles_wide >= sms / 2 && m_rows / 256 >= static_cast<long long>(pair_tiles) * num_groups &&
+              inter > out_cols_wide / 2;
   }
   *half = *pair ? 128 : (inter <= out_cols_wide / 2 || m_rows / 128 * tiles_wide < 2ll * sms) ? 64 : 128;
 }
@@ -690,7 +694,7 @@ static int gated_forward(const void* a, const void* w13, void* h, void* gu, void
   const int ctas = num_sms > 0 && num_sms < sms ? num_sms : sms;
   bool pair;
   int half;
-  gated_form(m_rows, num_groups, masked_stride, inter, 128, ctas, &pair, &half);
+  gated_form(m_rows, num_groups, masked_stride, inter, 128, gu ? 1 : 4, ctas, &pair, &half);
   const CUtensorMapDataType dt = dtype == 1 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   const int a_box = a_box_rows(m_rows, num_groups, pair);
   GatedMaps t = {};
@@ -748,7 +752,7 @@ static int gated_backward(const void* dy, const void* w2, const void* gu, const 
   const int ctas = num_sms > 0 && num_sms < sms ? num_sms : sms;
   bool pair;
   int half;
-  gated_form(m_rows, num_groups, 0, inter, 256, ctas, &pair, &half);
+  gated_form(m_rows, num_groups, 0, inter, 256, 1, ctas, &pair, &half);
   const CUtensorMapDataType dt = dtype == 1 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   const int a_box = a_box_rows(m_rows, num_groups, pair);
   GatedMaps t = {};
