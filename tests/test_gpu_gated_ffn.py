@@ -206,6 +206,58 @@ def test_single_gradients_strides_and_offsets():
     assert torch.equal(xt.grad, ones[1]) and torch.equal(w13t.grad, ones[2])
 
 
+def test_broadcast_inputs_sum_their_gradients():
+    """One token's row in every row of x, one expert's weights in every expert: the gradients of the shared tensors are
+    the sums over the copies (of 16-bit gradients, which autograd adds up)."""
+    sizes, hidden, inter = [20, 0, 45], 64, 48
+    x1, w13, w2, _ = _inputs([1, 0, 0], hidden, inter, 0, torch.bfloat16, seed=37)
+    dy = _inputs(sizes, hidden, inter, 0, torch.bfloat16, seed=38)[3]
+    s = torch.tensor(sizes, device=DEV)
+    leaves = [t.detach().clone().requires_grad_() for t in (x1, w13[:1], w2[:1])]
+    y = grouped_gated_ffn(leaves[0].expand(65, -1), leaves[1].expand(3, -1, -1), leaves[2].expand(3, -1, -1), s)
+    got = torch.autograd.grad(y, leaves, dy)
+    full = _run(x1.expand(65, -1).contiguous(), w13[:1].expand(3, -1, -1).contiguous(), w2[:1].expand(3, -1, -1).contiguous(),
+                sizes, "silu", dy)[1:]
+    for a, b in zip(got, full):
+        want = b.double().sum(0, keepdim=True)
+        assert ((a.double() - want).abs() <= 2.0 ** -8 * b.double().abs().sum(0, keepdim=True)).all()
+
+
+def test_two_threads_at_once():
+    """Calls from several host threads, each on its own stream."""
+    import threading
+
+    cases = [(_inputs(sz, 128, 96, 1, torch.bfloat16, seed=i), sz) for i, sz in enumerate(([40, 0, 9], [1, 2, 3], [0, 0, 70], [33, 33, 33]))]
+    want = [_run(x, w13, w2, sz, "silu", dy) for (x, w13, w2, dy), sz in cases]
+    torch.cuda.synchronize()
+    got = [None] * len(cases)
+
+    def work(i):
+        st = torch.cuda.Stream()
+        with torch.cuda.stream(st):
+            for _ in range(5):
+                (x, w13, w2, dy), sz = cases[i]
+                got[i] = _run(x, w13, w2, sz, "silu", dy)
+        st.synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(cases))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for a, b in zip(got, want):
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
+    assert _lib.device_status() == 0
+
+
+def test_fewer_sms():
+    sizes, hidden, inter, extra = SHAPES["straddling_block"]
+    x, w13, _, _ = _inputs(sizes, hidden, inter, extra, torch.bfloat16, seed=41)
+    s = torch.tensor(sizes, device=DEV)
+    n = sum(sizes)
+    assert torch.equal(m_grouped_gated_gemm(x, w13, s, numSM=3)[:n], m_grouped_gated_gemm(x, w13, s)[:n])
+
+
 def test_repeatable_and_on_other_streams():
     sizes, hidden, inter, extra = SHAPES["straddling_block"]
     x, w13, w2, dy = _inputs(sizes, hidden, inter, extra, torch.bfloat16, seed=19)

@@ -132,6 +132,22 @@ def test_weights_in_16_bits_and_views():
     assert torch.equal(got, xt[plan.send_order // 2])
 
 
+def test_second_derivatives_are_refused():
+    _, plan = _plan(6, 2, 8, seed=1)
+    x = torch.randn(6, 16, device=DEV).bfloat16().requires_grad_()
+    rows = permute_rows(x, plan.pos, plan.send_order, 2)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(rows.sum(), x, create_graph=True)
+    w = torch.rand(6, 2, device=DEV).requires_grad_()
+    out = combine_rows(rows.detach(), w, plan.pos, plan.send_order)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(out.float().sum(), w, create_graph=True)
+    w13, w2 = _layer(8, 16, 8, torch.bfloat16, 3)
+    y = moe_ffn(x, torch.zeros(6, 1, dtype=torch.int64, device=DEV), torch.ones(6, 1, device=DEV), w13.requires_grad_(), w2)
+    with pytest.raises(RuntimeError, match="differentiable once|differentiate twice"):
+        torch.autograd.grad(torch.autograd.grad(y.float().sum(), w13, create_graph=True)[0].float().sum(), w13)
+
+
 # ------------------------------------------------------------------------------------------- the operators together
 def _layer(experts, hidden, inter, dtype, seed):
     gen = torch.Generator(device=DEV).manual_seed(seed)

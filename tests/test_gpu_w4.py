@@ -151,6 +151,22 @@ def test_no_rows():
     assert torch.all(out == 5.0) and _lib.device_status() == 0
 
 
+def test_fewer_sms_and_concurrent_streams():
+    b = _weights(6, 200, 512, 64, True, torch.bfloat16)
+    sizes = torch.tensor([3, 0, 20, 1, 0, 9], device=DEV)
+    a = _activations(33, 512, torch.bfloat16)
+    want = m_grouped_gemm_w4(a, b, sizes)
+    assert torch.equal(m_grouped_gemm_w4(a, b, sizes, num_sms=2), want)
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(3):
+        st = torch.cuda.Stream()
+        with torch.cuda.stream(st):
+            got += [m_grouped_gemm_w4(a, b, sizes) for _ in range(4)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want) for g in got) and _lib.device_status() == 0
+
+
 def test_scales_off_every_alignment():
     """Scales and zeros that begin 2 and 1 bytes off 16, an odd number of groups per row."""
     g, rows, k, gs = 2, 50, 96, 32

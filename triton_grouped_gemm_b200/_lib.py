@@ -153,7 +153,7 @@ def require_cuda(*tensors: torch.Tensor) -> None:
 
 def stream_ptr(device: torch.device) -> int:
     # the raw handle, without a Stream object around it (2.2 us of a call)
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if device.index is None else device.index)
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice() if device.index is None else device.index)
 
 
 _no_guard = contextlib.nullcontext()
@@ -161,7 +161,7 @@ _no_guard = contextlib.nullcontext()
 
 def on_device(device: torch.device):
     """``with on_device(t.device):`` - a device guard that costs nothing where that device is current already."""
-    return _no_guard if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return _no_guard if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
 def ptr(t: torch.Tensor) -> int:

@@ -11,19 +11,27 @@ unpermute).
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from ..gemm.autograd import grouped_gated_ffn
 from .dispatch import make_plan
 
 
-def _check_plan(what: str, pos: torch.Tensor, order: torch.Tensor, pairs: int, device) -> None:
+def _check_plan(what: str, rows: torch.Tensor, pos: torch.Tensor, order: torch.Tensor, pairs: int) -> None:
+    assert rows.dtype in (torch.bfloat16, torch.float16), f"{what}: data type {rows.dtype} not supported"
     assert pos.dtype == torch.int64 and order.dtype == torch.int64, f"{what}: pos and order must be int64"
     assert pos.numel() == pairs and pos.is_contiguous() and order.is_contiguous() and order.dim() == 1, \
         f"{what}: pos must hold one contiguous entry per (token, k) pair and order one per row"
-    _lib.require_cuda(pos, order)
-    assert pos.device == device and order.device == device, f"{what}: all operands must be on one device"
+    _lib.require_cuda(rows, pos, order)
+    device = rows.get_device()
+    assert pos.get_device() == device and order.get_device() == device, f"{what}: all operands must be on one device"
+
+
+def _once(what: str) -> None:
+    # autograd calls backward with gradients enabled only to differentiate it again, which these kernels cannot
+    # (cheaper than once_differentiable's wrapper, 3 us of a call)
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{what} is differentiable once: create_graph=True is not supported")
 
 
 def _permute(x, pos, order, top_k):
@@ -55,8 +63,8 @@ class _PermuteRows(torch.autograd.Function):
         return _permute(x, pos, order, top_k)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, drows):
+        _once("permute_rows")
         pos, order = ctx.saved_tensors
         return _combine(_lib.aligned(drows), None, pos, order, pos.numel() // ctx.top_k, ctx.top_k), None, None, None
 
@@ -71,8 +79,8 @@ class _CombineRows(torch.autograd.Function):
         return _combine(rows, w32, pos, order, t, top_k)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dout):
+        _once("combine_rows")
         rows, w32, pos, order = ctx.saved_tensors
         dout = _lib.aligned(dout)
         t, h = dout.shape
@@ -91,11 +99,9 @@ def permute_rows(x: torch.Tensor, pos: torch.Tensor, order: torch.Tensor, top_k:
     """x [T, H] bf16 / fp16 -> rows [R, H] with ``rows[pos[t * top_k + j]] = x[t]`` (R = order.numel()), differentiable
     in x.  H a multiple of 8, top_k <= 32."""
     assert x.dim() == 2, "x must be 2D [T, H]"
-    _lib.dtype_code(x.dtype)
-    _lib.require_cuda(x)
-    _check_plan("permute_rows", pos, order, x.shape[0] * top_k, x.device)
+    _check_plan("permute_rows", x, pos, order, x.shape[0] * top_k)
     x = x.contiguous()
-    if torch.is_grad_enabled() and x.requires_grad:
+    if x.requires_grad and torch.is_grad_enabled():
         return _PermuteRows.apply(x, pos, order, top_k)
     return _permute(x, pos, order, top_k)
 
@@ -106,12 +112,10 @@ def combine_rows(rows: torch.Tensor, topk_weight: torch.Tensor, pos: torch.Tenso
     assert rows.dim() == 2 and topk_weight.dim() == 2, "rows must be 2D [R, H] and topk_weight 2D [T, k]"
     assert topk_weight.is_floating_point(), "topk_weight must be floating point"
     assert order.numel() == rows.shape[0], "order must have one entry per row"
-    _lib.dtype_code(rows.dtype)
-    _lib.require_cuda(rows, topk_weight)
-    assert topk_weight.device == rows.device, "combine_rows: all operands must be on one device"
-    _check_plan("combine_rows", pos, order, topk_weight.numel(), rows.device)
+    _check_plan("combine_rows", rows, pos, order, topk_weight.numel())
+    assert topk_weight.get_device() == rows.get_device(), "combine_rows: all operands must be on one device"
     rows = rows.contiguous()
-    if torch.is_grad_enabled() and (rows.requires_grad or topk_weight.requires_grad):
+    if (rows.requires_grad or topk_weight.requires_grad) and torch.is_grad_enabled():
         return _CombineRows.apply(rows, topk_weight, pos, order)
     t, top_k = topk_weight.shape
     return _combine(rows, topk_weight.to(torch.float32).contiguous(), pos, order, t, top_k)
