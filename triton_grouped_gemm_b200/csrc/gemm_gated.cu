@@ -18,6 +18,12 @@
 //   * Everything else is the M-grouped kernel's: persistent CTAs, one walk over the group sizes, TMA ring, one MMA
 //     issuer, two accumulators, epilogue warps that store through swizzled staging buffers.
 //
+// Measured with 655 360 rows over 128 groups, K 2048, I 768, beside the plain M-grouped product of the same shape on
+// the same GPU: forward 2.78 ms (2.72), keeping g and u 3.26 ms (3.38 - the same, both at the power limit), gradient
+// 1.94 ms (1.66; it reads 2.0 GB and writes 2.0 GB where the plain product writes 1.0 GB).  With integer arithmetic for
+// the codes and an exactly rounded reciprocal they took 3.96 and 3.54 ms: the epilogue, not the tensor cores, was the
+// bound.  With 128 rows over 80 of 128 groups the forward is bound by the weights: 503 MB in 89 us, 5.65 TB/s.
+//
 // Rows behind the last group have no product; the epilogue warps zero them in `tail` (the layer's output in the
 // forward call, its input gradient in the backward call) once their tiles are done.
 #include <cuda_bf16.h>

@@ -11,7 +11,10 @@
 //
 // All three kernels are bound by HBM bytes: a token's vector is read once, whatever its top_k, and a row is
 // read or written once.  One warp (few tokens: one block) takes a token and walks its columns in 16-byte vectors
-// with the loads of its top_k rows in flight together.  Sums and dot products are fp32, rounded once.
+// with the loads of its top_k rows in flight together.  Sums and dot products are fp32, rounded once.  Measured, 81 920
+// tokens, top-8, hidden 2048 (share of the measured copy bandwidth, 6569 GB/s): permute 504 us (0.91), combine and the
+// gradient of permute 455 us (1.01; 868 us with the rows' addresses shuffled anew for every vector), the gradients of
+// combine 1000 us (0.87).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

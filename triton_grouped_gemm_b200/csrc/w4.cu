@@ -6,7 +6,7 @@
 // weights' bytes, N * K / 2 per expert that has a row; the arithmetic only has to keep up with them:
 //
 //   * a 4-bit value becomes a 16-bit one by OR-ing it into the mantissa of a power of two (128 + q in bf16,
-//     1024 + q in fp16) and subtracting 128 + zero (1024 + zero): exact, 1.4 instructions per value.
+//     1024 + q in fp16) and subtracting 128 + zero (1024 + zero): exact, 1.4 instructions per value (fp16: 1.1).
 //   * products run on mma.sync m16n8k16 with the WEIGHTS as the 16-row operand and up to 8 rows of `a` as the
 //     8 columns.  tcgen05 has no use here: its smallest tile is 64 rows of `a` or of weights staged through
 //     shared memory in 16 bits, four times the bytes that bound this kernel.
@@ -21,9 +21,16 @@
 // depend on timing.  Blocks are persistent over the (expert with rows, tile, row chunk) items; an expert's row chunks
 // are neighbours, so the second one finds the weights in L2.  Of four further warps one fetches the stages by TMA and
 // three the scales, all running ahead across the items' borders, so a block never drains, and the multiplying warps
-// meet only to join their sums.  The 128-byte swizzle makes both operands' fragment loads free of bank conflicts (rows of `a` are taken in
-// the order 0 4 1 5 2 6 3 7 for that).  With the loads off the warps' hands the kernel is bound by the logic
-// pipe (masks, shifts, byte permutes: 24 instructions per 32 x 32 values in fp16, 32 in bf16) until HBM takes over.
+// meet only to join their sums.  The 128-byte swizzle makes both operands' fragment loads free of bank conflicts (rows
+// of `a` are taken in the order 0 4 1 5 2 6 3 7 for that).
+//
+// What bounds it now is issue: per 32 x 32 weights some 24 (bf16: 32) instructions of the half-rate logic pipe, 20 of
+// the others, and as many again around them.  Measured (time, share of the floor of the weights' bytes at the copy
+// bandwidth): 256 rows over 112 of 128 experts, gated, K 4096, 1024 + 1024 columns, fp16 with zeros 118 us, 0.64;
+// the same in bf16 128 us, 0.59; 256 rows, K 768, 2048 columns, groups of 64 with zeros 39 us, 0.38; one token's eight
+// experts, K 2048, 768 + 768 columns 10 us a launch, of which 1 us is the walk over the sizes, 1-2 the first bytes'
+// way, 3 the products and the rest the launch.  Splitting the stage finer (half the k per warp and stage, three
+// blocks per SM) took 174 us where this takes 118, one block of 16 warps 121.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -106,17 +113,6 @@ __device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t m
   return r;
 }
 
-template <bool kFp16>
-__device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
-  if constexpr (kFp16) {
-    const __half2 d = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&d);
-  } else {
-    const __nv_bfloat162 d = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&d);
-  }
-}
-
 // magic + zero in both halves: 0x43zz is 128 + zz in bf16 (zz < 128), 0x64zz is 1024 + zz in fp16
 template <bool kFp16>
 __device__ __forceinline__ uint32_t zero_pair(uint32_t zero) {
@@ -142,7 +138,11 @@ __device__ __forceinline__ void unpack_word(uint32_t w, uint32_t zp, uint32_t (&
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) p[i] = sub2<false>(and_or(w >> (4 * i), 0x000F000Fu, 0x43004300u), zp);
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t q = and_or(w >> (4 * i), 0x000F000Fu, 0x43004300u);
+      const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&q), *reinterpret_cast<__nv_bfloat162*>(&zp));
+      p[i] = *reinterpret_cast<const uint32_t*>(&d);
+    }
   }
 }
 
