@@ -14,7 +14,7 @@
 // with the loads of its top_k rows in flight together.  Sums and dot products are fp32, rounded once.  Measured, 81 920
 // tokens, top-8, hidden 2048 (share of the measured copy bandwidth, 6569 GB/s): permute 504 us (0.91), combine and the
 // gradient of permute 455 us (1.01; 868 us with the rows' addresses shuffled anew for every vector), the gradients of
-// combine 1000 us (0.87).
+// combine 909 us (0.95).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -193,9 +193,10 @@ combine_rows_kernel(const uint4* __restrict__ rows, const long long* __restrict_
 }
 
 // drows[pos[t,j]] = w[t,j] * dout[t] and dw[t,j] = <dout[t], rows[pos[t,j]]> in one pass over the rows; drows or dw
-// may be nullptr (that gradient is not wanted).  A pair without a row has dw = 0.
+// may be nullptr (that gradient is not wanted).  A pair without a row has dw = 0.  Five blocks per SM: left alone the
+// compiler takes 145 registers, three blocks and 1000 us for the case above; 4, 5 and 6 blocks 926, 909 and 952 us.
 template <bool kSpread, int kK, bool kFp16>
-__global__ void __launch_bounds__(kRowsThreads)
+__global__ void __launch_bounds__(kRowsThreads, 5)
 combine_rows_grad_kernel(const uint4* __restrict__ dout, const uint4* __restrict__ rows,
                          const long long* __restrict__ pos, const long long* __restrict__ order,
                          const float* __restrict__ weights, uint4* __restrict__ drows, float* __restrict__ dweights,
