@@ -26,11 +26,12 @@
 //
 // What bounds it now is issue: per 32 x 32 weights some 24 (bf16: 32) instructions of the half-rate logic pipe, 20 of
 // the others, and as many again around them.  Measured (time, share of the floor of the weights' bytes at the copy
-// bandwidth): 256 rows over 112 of 128 experts, gated, K 4096, 1024 + 1024 columns, fp16 with zeros 118 us, 0.64;
-// the same in bf16 128 us, 0.59; 256 rows, K 768, 2048 columns, groups of 64 with zeros 39 us, 0.38; one token's eight
+// bandwidth): 256 rows over 112 of 128 experts, gated, K 4096, 1024 + 1024 columns, fp16 107 us, 0.69; the same in bf16
+// 116 us, with zeros 121 us, 0.62; 256 rows, K 768, 2048 columns, groups of 64 with zeros 38 us, 0.39; one token's eight
 // experts, K 2048, 768 + 768 columns 10 us a launch, of which 1 us is the walk over the sizes, 1-2 the first bytes'
-// way, 3 the products and the rest the launch.  Splitting the stage finer (half the k per warp and stage, three
-// blocks per SM) took 174 us where this takes 118, one block of 16 warps 121.
+// way, 3 the products and the rest the launch.  Each stage and warp has a fixed cost of about two blocks of 32 x 32, so
+// a warp gets 8 (kNT = 2: 4) of a stage: the first case took 174 us at 2 of them, 115 at 4; 16 warps in one block
+// per SM took 121, 64 rows per warp spilled.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -42,9 +43,9 @@
 
 namespace b200 {
 
-constexpr int kW4WindowGroups = 32;   // scales are staged for this many groups at a time
-constexpr int kW4ScalePitch = 80;     // bytes per row of the staged scales / zeros: odd numbers of 16-byte units,
-constexpr int kW4ZeroPitch = 48;      // so that 8 rows lie in 8 different banks
+constexpr int kW4WindowGroups = 16;   // scales are staged for this many groups at a time
+constexpr int kW4ScalePitch = 48;     // bytes per row of the staged scales / zeros: odd numbers of 16-byte units,
+constexpr int kW4ZeroPitch = 16;      // so that 8 rows lie in 8 different banks
 constexpr int kW4MaxGroups = 1024;    // experts
 
 struct W4Args {
@@ -765,8 +766,8 @@ static int w4_m_grouped(const void* a, const void* w4, const void* scale, const 
   const long long rows_at_most = m_rows < num_groups ? m_rows : num_groups;
   if (m_rows <= 8ll * num_groups && rows_at_most * ((gated ? 2ll * n : n) / 64) <= 2ll * want)
     return form_w4<1, 8, 1, 3, 16>(o, p, log_gs, gated, dtype, want, stream);
-  return m_rows <= 8ll * num_groups ? form_w4<4, 2, 1, 3, 8>(o, p, log_gs, gated, dtype, want, stream)
-                                    : form_w4<2, 4, 2, 4, 8>(o, p, log_gs, gated, dtype, want, stream);
+  return m_rows <= 8ll * num_groups ? form_w4<4, 2, 1, 2, 16>(o, p, log_gs, gated, dtype, want, stream)
+                                    : form_w4<4, 2, 2, 3, 8>(o, p, log_gs, gated, dtype, want, stream);
 }
 
 static int w4_quant(const void* w, void* q, void* scale, void* zero, int64_t rows, int k, int group_size, int dtype,
