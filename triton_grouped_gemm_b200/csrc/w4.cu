@@ -8,8 +8,11 @@
 //   * a 4-bit value becomes a 16-bit one by OR-ing it into the mantissa of a power of two (128 + q in bf16,
 //     1024 + q in fp16) and subtracting 128 + zero (1024 + zero): exact, 1.4 instructions per value (fp16: 1.1).
 //   * products run on mma.sync m16n8k16 with the WEIGHTS as the 16-row operand and up to 8 rows of `a` as the
-//     8 columns.  tcgen05 has no use here: its smallest tile is 64 rows of `a` or of weights staged through
-//     shared memory in 16 bits, four times the bytes that bound this kernel.
+//     8 columns.  tcgen05 wants the weights in 16 bits in shared memory (four times the bytes that bound this kernel)
+//     or in tensor memory.  The latter was built - 128 weight rows unpacked into tensor memory by two warpgroups,
+//     16 or 48 rows of `a`, a group's sums read back, scaled and added up by a third - and was slower: the three
+//     hand-overs per 128 k take 0.8 us where this takes 0.3 (first case below 172 us against 113; 36 rows per expert,
+//     groups of 32: 82 against 84).
 //   * q - zero is a whole number, so the products of a group are summed unscaled (fp32) and the scale enters once
 //     per group and output: the only rounding is that of the result.
 //   * eight neighbouring k of a row are one 32-bit word; the pairs that mask and shift take out of it are (0,4)
