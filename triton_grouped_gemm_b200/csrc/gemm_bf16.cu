@@ -42,7 +42,7 @@ template <int kBlockN, int kStages, bool kBMnMajor, bool kFp8>
 __global__ void __launch_bounds__(kNumThreads, 1)
 m_grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
                  const __grid_constant__ CUtensorMap tm_c, void* __restrict__ c_ptr, const void* __restrict__ sizes, int sizes_i64, int num_groups,
-                 int masked_stride, long long m_rows, int n, int k, int in_fmt, int out_fp16, int a_box,
+                 int masked_stride, long long m_rows, int n, int k, int in_fmt, int out_fp16,
                  const float* __restrict__ a_scale, const float* __restrict__ b_scale, unsigned* status) {
   static_assert(!(kFp8 && kBMnMajor), "fp8 operands are K-major only");
   constexpr int kElemsPerKb = kFp8 ? 128 : 64;
@@ -103,8 +103,6 @@ m_grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
       if (!w.seek(mt)) break;
       const int row0 = static_cast<int>(w.tile_row0(mt));
       const int g = w.g;
-      // only the boxes that hold rows of the group; the others' lanes multiply what lies there and are not stored
-      const int a_boxes = (min(kBlockM, static_cast<int>(w.group_row_end()) - row0) + a_box - 1) / a_box;
       for (int kb = 0; kb < num_kb; ++kb) {
         if (!wait_bounded(empty_bar(stage), phase ^ 1u, abort_flag, status, kDevTimeoutProducer)) {
           ok = false;
@@ -113,9 +111,8 @@ m_grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
         if (lane == 0) {
           const uint32_t a_dst = smem_base + stage * L::kStageBytes;
           const uint32_t b_dst = a_dst + L::kABytes;
-          mbar_arrive_expect_tx(full_bar(stage), a_boxes * a_box * 128 + L::kBBytes);
-          for (int i = 0; i < a_boxes; ++i)
-            tma_load_2d(a_dst + i * a_box * 128, &tm_a, full_bar(stage), kb * kElemsPerKb, row0 + i * a_box);
+          mbar_arrive_expect_tx(full_bar(stage), L::kStageBytes);
+          tma_load_2d(a_dst, &tm_a, full_bar(stage), kb * kElemsPerKb, row0);
           if constexpr (!kBMnMajor) {
             tma_load_3d(b_dst, &tm_b, full_bar(stage), kb * kElemsPerKb, nt * kBlockN, g);
           } else {
@@ -242,14 +239,14 @@ template <int kBlockN, int kStages, bool kBMnMajor, bool kFp8>
 static int launch_m_grouped(const CUtensorMap& tm_a, const CUtensorMap& tm_b, const CUtensorMap& tm_c, void* c,
                             const void* sizes,
                             int sizes_is_i64, int num_groups, int masked_stride, long long m_rows, int n, int k,
-                            int in_fmt, int out_fp16, int a_box, const float* a_scale, const float* b_scale, int grid,
+                            int in_fmt, int out_fp16, const float* a_scale, const float* b_scale, int grid,
                             cudaStream_t stream) {
   using L = MGroupedSmem<kBlockN, kStages>;
   auto kern = m_grouped_kernel<kBlockN, kStages, kBMnMajor, kFp8>;
   B200_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kDynamicBytes));
   unsigned* status = device_status_ptr();
   kern<<<grid, kNumThreads, L::kDynamicBytes, stream>>>(tm_a, tm_b, tm_c, c, sizes, sizes_is_i64, num_groups, masked_stride,
-                                                        m_rows, n, k, in_fmt, out_fp16, a_box, a_scale, b_scale, status);
+                                                        m_rows, n, k, in_fmt, out_fp16, a_scale, b_scale, status);
   B200_CUDA(cudaGetLastError());
   return 0;
 }
@@ -303,13 +300,12 @@ static int m_grouped_common(const void* a, const void* b, void* c, const void* s
   const bool pair = (masked_stride > 0 && g_cta_pair_mode != 1) ? false : want_pair(m_rows, num_groups, n, grid, block_n);
   if (pair) block_n = 128;  // per-CTA slice of the 256-wide pair tile (tensor-map box rows)
 
-  const int a_box = masked_stride == 0 ? a_box_rows(m_rows, num_groups, pair) : kBlockM;
   const CUtensorMapDataType dt = dtype == 1 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   CUtensorMap tm_a, tm_b;
   {
     const uint64_t dims[2] = {static_cast<uint64_t>(k), static_cast<uint64_t>(m_rows)};
     const uint64_t strides[1] = {static_cast<uint64_t>(k) * 2};
-    const uint32_t box[2] = {kBlockK, static_cast<uint32_t>(a_box)};
+    const uint32_t box[2] = {kBlockK, kBlockM};
     int rc = encode_tmap(&tm_a, dt, 2, a, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, "A");
     if (rc) return rc;
   }
@@ -347,9 +343,9 @@ static int m_grouped_common(const void* a, const void* b, void* c, const void* s
   }
 #define B200_LAUNCH(BN, ST)                                                                                          \
   (trans_b ? launch_m_grouped<BN, ST, false, false>(tm_a, tm_b, tm_c, c, sizes, sizes_is_i64, num_groups, masked_stride, m_rows, n, \
-                                                    k, in_fmt, dtype, a_box, nullptr, nullptr, grid, stream)         \
+                                                    k, in_fmt, dtype, nullptr, nullptr, grid, stream)         \
            : launch_m_grouped<BN, ST, true, false>(tm_a, tm_b, tm_c, c, sizes, sizes_is_i64, num_groups, masked_stride, m_rows, n,  \
-                                                   k, in_fmt, dtype, a_box, nullptr, nullptr, grid, stream))
+                                                   k, in_fmt, dtype, nullptr, nullptr, grid, stream))
   if (block_n == 256) return B200_LAUNCH(256, 4);
   if (block_n == 128) return B200_LAUNCH(128, 6);
   return B200_LAUNCH(64, 8);
@@ -416,7 +412,7 @@ static int fp8_rowcol_m_grouped(const void* a, const float* a_scale, const void*
                                               (num_sms > 0 && num_sms < sms) ? num_sms : 0, stream);
 #define B200_LAUNCH8(BN, ST)                                                                                        \
   launch_m_grouped<BN, ST, false, true>(tm_a, tm_b, tm_c, c, sizes, sizes_is_i64, num_groups, 0, m_rows, n, k, in_fmt, out_dtype, \
-                                        kBlockM, a_scale, b_scale, grid, stream)
+                                        a_scale, b_scale, grid, stream)
   if (block_n == 256) return B200_LAUNCH8(256, 4);
   if (block_n == 128) return B200_LAUNCH8(128, 6);
   return B200_LAUNCH8(64, 8);

@@ -141,7 +141,6 @@ struct GatedArgs {
   long long m_rows;
   int inter;          // I
   int k;
-  int a_box;          // rows of a TMA box of A: 128, or 32 where groups are short (see a_box_rows)
   int in_fmt;         // UMMA operand format: 0 = f16, 1 = bf16
   int act;
   uint16_t* h;        // forward: [m_rows, I]
@@ -232,8 +231,6 @@ gated_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ C
       if (!w.seek(mt)) break;
       const int row0 = static_cast<int>(w.tile_row0(mt)) + static_cast<int>(rank) * 128;
       const int g = w.g;
-      // only the boxes that hold rows of the group; the others' lanes multiply what lies there and are not stored
-      const int a_boxes = (min(128, static_cast<int>(w.group_row_end()) - row0) + p.a_box - 1) / p.a_box;
       for (int kb = 0; kb < num_kb; ++kb) {
         if (!wait_bounded(empty_bar(stage), phase ^ 1u, abort_flag, p.status, kDevTimeoutProducer)) {
           ok = false;
@@ -256,9 +253,8 @@ gated_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ C
                                  nt * kOutCols + static_cast<int>(rank) * 128 + j * 64, kb * kBlockK, g);
             }
           } else {
-            mbar_arrive_expect_tx(full_bar(stage), a_boxes * p.a_box * 128 + L::kBBytes);
-            for (int i = 0; i < a_boxes; ++i)
-              tma_load_2d(a_dst + i * p.a_box * 128, &tm_a, full_bar(stage), kb * kBlockK, row0 + i * p.a_box);
+            mbar_arrive_expect_tx(full_bar(stage), L::kStageBytes);
+            tma_load_2d(a_dst, &tm_a, full_bar(stage), kb * kBlockK, row0);
             if constexpr (!kBwd) {
               tma_load_4d(b_dst, &tm_b, full_bar(stage), kb * kBlockK, nt * kHalf, 0, g);
               tma_load_4d(b_dst + kHalf * 128, &tm_b, full_bar(stage), kb * kBlockK, nt * kHalf, 1, g);
@@ -702,9 +698,8 @@ static int gated_forward(const void* a, const void* w13, void* h, void* gu, void
   int half;
   gated_form(m_rows, num_groups, masked_stride, inter, 128, gu ? 1 : 4, ctas, &pair, &half);
   const CUtensorMapDataType dt = dtype == 1 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  const int a_box = a_box_rows(m_rows, num_groups, pair);
   GatedMaps t = {};
-  if (int rc = rows_map(&t.a, dt, a, m_rows, k, a_box, "A")) return rc;
+  if (int rc = rows_map(&t.a, dt, a, m_rows, k, 128, "A")) return rc;
   {
     const uint64_t ku = static_cast<uint64_t>(k), iu = static_cast<uint64_t>(inter);
     const uint64_t dims[4] = {ku, iu, 2, static_cast<uint64_t>(num_groups)};
@@ -723,7 +718,6 @@ static int gated_forward(const void* a, const void* w13, void* h, void* gu, void
   p.m_rows = m_rows;
   p.inter = inter;
   p.k = k;
-  p.a_box = a_box;
   p.in_fmt = dtype == 1 ? 0 : 1;
   p.act = act;
   p.h = static_cast<uint16_t*>(h);
@@ -760,9 +754,8 @@ static int gated_backward(const void* dy, const void* w2, const void* gu, const 
   int half;
   gated_form(m_rows, num_groups, 0, inter, 256, 1, ctas, &pair, &half);
   const CUtensorMapDataType dt = dtype == 1 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  const int a_box = a_box_rows(m_rows, num_groups, pair);
   GatedMaps t = {};
-  if (int rc = rows_map(&t.a, dt, dy, m_rows, k, a_box, "dY")) return rc;
+  if (int rc = rows_map(&t.a, dt, dy, m_rows, k, 128, "dY")) return rc;
   {
     const uint64_t ku = static_cast<uint64_t>(k), iu = static_cast<uint64_t>(inter);
     const uint64_t dims[3] = {iu, ku, static_cast<uint64_t>(num_groups)};
@@ -779,7 +772,6 @@ static int gated_backward(const void* dy, const void* w2, const void* gu, const 
   p.m_rows = m_rows;
   p.inter = inter;
   p.k = k;
-  p.a_box = a_box;
   p.in_fmt = dtype == 1 ? 0 : 1;
   p.act = act;
   p.exps = const_cast<uint8_t*>(static_cast<const uint8_t*>(exps));

@@ -129,13 +129,6 @@ __device__ __forceinline__ void store_zero_row_16bit(uint16_t* c_row, bool row_o
     *reinterpret_cast<uint4*>(c_row + col) = make_uint4(0, 0, 0, 0);
 }
 
-// Rows of a TMA box of A in the single-CTA kernels.  Where groups hold few rows a tile's 128 rows of A are mostly other
-// groups' rows, fetched from L2 beside the weights the call is bound by; boxes of 32 rows leave them out (decoding,
-// 128 rows over 80 of 128 experts, K 2048: gate+up tile traffic 1.0 -> 0.63 GB).  Long groups keep one box per stage.
-inline int a_box_rows(long long m_rows, int num_groups, bool pair) {
-  return !pair && m_rows < 64ll * num_groups ? 32 : 128;
-}
-
 // CTA-pair (cta_group::2) variant of the M-grouped kernels, 256 x 256 tiles (gemm_pair.cu).
 // `want_ctas` <= 0: as many CTAs as are co-resident.  tm_b must describe 128-row (K-major) or
 // 64 x 64 (MN-major) boxes; tm_a 128-row boxes; tm_c 32 x 64 boxes.

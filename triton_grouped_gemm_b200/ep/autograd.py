@@ -125,7 +125,9 @@ def moe_ffn(x: torch.Tensor, topk_idx: torch.Tensor, topk_weight: torch.Tensor, 
             activation: str = "silu") -> torch.Tensor:
     """Trainable 16-bit MoE feed-forward layer on one rank: x [T, H], topk_idx [T, k] (an id outside the experts drops
     the pair), topk_weight [T, k], w13 [E, 2*I, H] (gate rows, then up rows), w2 [E, H, I] -> [T, H], with gradients
-    for x, topk_weight, w13 and w2.  Nothing synchronises the host."""
+    for x, topk_weight, w13 and w2.  Nothing synchronises the host.  The plan leaves the order of the rows inside an
+    expert open: it changes nothing in the output or the gradients of x and topk_weight, but the weights' gradients sum
+    over the rows and may differ in their last bits from one call to the next."""
     top_k = topk_idx.shape[1]
     plan = make_plan(topk_idx, w13.shape[0])
     rows = permute_rows(x, plan.pos, plan.send_order, top_k)
