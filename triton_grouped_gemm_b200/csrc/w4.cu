@@ -29,8 +29,8 @@
 //
 // What bounds it now is issue: per 32 x 32 weights some 24 (bf16: 32) instructions of the half-rate logic pipe, 20 of
 // the others, and as many again around them.  Measured (time, share of the floor of the weights' bytes at the copy
-// bandwidth): 256 rows over 112 of 128 experts, gated, K 4096, 1024 + 1024 columns, fp16 107 us, 0.69; the same in bf16
-// 116 us, with zeros 121 us, 0.62; 256 rows, K 768, 2048 columns, groups of 64 with zeros 38 us, 0.39; one token's eight
+// bandwidth): 256 rows over 112 of 128 experts, gated, K 4096, 1024 + 1024 columns, fp16 with zeros 109 us, 0.69; the
+// same in bf16 116 us, with zeros 121 us, 0.62; 256 rows, K 768, 2048 columns, groups of 64 with zeros 38 us, 0.39; one token's eight
 // experts, K 2048, 768 + 768 columns 10 us a launch, of which 1 us is the walk over the sizes, 1-2 the first bytes'
 // way, 3 the products and the rest the launch.  Each stage and warp has a fixed cost of about two blocks of 32 x 32, so
 // a warp gets 8 (kNT = 2: 4) of a stage: the first case took 174 us at 2 of them, 115 at 4; 16 warps in one block
