@@ -89,6 +89,7 @@ m_grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_holder;
+  chain_wait();
 
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
@@ -245,9 +246,8 @@ static int launch_m_grouped(const CUtensorMap& tm_a, const CUtensorMap& tm_b, co
   auto kern = m_grouped_kernel<kBlockN, kStages, kBMnMajor, kFp8>;
   B200_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kDynamicBytes));
   unsigned* status = device_status_ptr();
-  kern<<<grid, kNumThreads, L::kDynamicBytes, stream>>>(tm_a, tm_b, tm_c, c, sizes, sizes_is_i64, num_groups, masked_stride,
-                                                        m_rows, n, k, in_fmt, out_fp16, a_scale, b_scale, status);
-  B200_CUDA(cudaGetLastError());
+  B200_CUDA(launch_chained(kern, grid, kNumThreads, L::kDynamicBytes, stream, tm_a, tm_b, tm_c, c, sizes, sizes_is_i64,
+                           num_groups, masked_stride, m_rows, n, k, in_fmt, out_fp16, a_scale, b_scale, status));
   return 0;
 }
 

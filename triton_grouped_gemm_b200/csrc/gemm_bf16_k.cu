@@ -90,6 +90,8 @@ __global__ void __launch_bounds__(1024) k_grouped_plan_kernel(const void* __rest
                                                               const int* __restrict__ group_start,
                                                               const int* __restrict__ group_end, int num_groups,
                                                               int* __restrict__ scratch) {
+  chain_wait();
+  chain_release();
   int* starts = scratch + kPlanHeaderWords;
   int* tokens = starts + num_groups;
   int* order = tokens + num_groups;
@@ -188,6 +190,7 @@ k_grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_holder;
+  chain_wait();
 
   // tile -> (group slot, m tile, n tile): n fastest, so CTAs running side by side share A chunks.
   // Balanced mode visits the groups in the plan's order (most tokens first).
@@ -470,19 +473,15 @@ static int launch_k_grouped(const CUtensorMap& tm_a, const CUtensorMap& tm_b, co
     // balanced: plan (starts, token counts, longest-first order, zeroed tile counter), then the GEMM
     auto kern = k_grouped_kernel<kBlockN, kStages, kFp8, true>;
     B200_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kDynamicBytes));
-    k_grouped_plan_kernel<<<1, 1024, 0, stream>>>(sizes, sizes_is_i64, gs, ge, num_groups, scratch);
-    B200_CUDA(cudaGetLastError());
-    kern<<<grid, kNumThreads, L::kDynamicBytes, stream>>>(tm_a, tm_b, tm_c, c, sizes, sizes_is_i64, gs, ge, num_groups,
-                                                          m_dim, n_dim, k_total, in_fmt, out_fp16, a_scale, b_scale,
-                                                          scratch, status);
+    B200_CUDA(launch_chained(k_grouped_plan_kernel, 1, 1024, 0, stream, sizes, sizes_is_i64, gs, ge, num_groups, scratch));
+    B200_CUDA(launch_chained(kern, grid, kNumThreads, L::kDynamicBytes, stream, tm_a, tm_b, tm_c, c, sizes, sizes_is_i64, gs,
+                             ge, num_groups, m_dim, n_dim, k_total, in_fmt, out_fp16, a_scale, b_scale, scratch, status));
   } else {
     auto kern = k_grouped_kernel<kBlockN, kStages, kFp8, false>;
     B200_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kDynamicBytes));
-    kern<<<grid, kNumThreads, L::kDynamicBytes, stream>>>(tm_a, tm_b, tm_c, c, sizes, sizes_is_i64, gs, ge, num_groups,
-                                                          m_dim, n_dim, k_total, in_fmt, out_fp16, a_scale, b_scale,
-                                                          nullptr, status);
+    B200_CUDA(launch_chained(kern, grid, kNumThreads, L::kDynamicBytes, stream, tm_a, tm_b, tm_c, c, sizes, sizes_is_i64, gs,
+                             ge, num_groups, m_dim, n_dim, k_total, in_fmt, out_fp16, a_scale, b_scale, nullptr, status));
   }
-  B200_CUDA(cudaGetLastError());
   return 0;
 }
 
@@ -513,8 +512,7 @@ static bool want_k_pair(const int* scratch, int num_groups, int m_dim, int n_dim
 
 static int launch_plan(const void* sizes, int sizes_is_i64, const int* gs, const int* ge, int num_groups, int* scratch,
                        cudaStream_t stream) {
-  k_grouped_plan_kernel<<<1, 1024, 0, stream>>>(sizes, sizes_is_i64, gs, ge, num_groups, scratch);
-  B200_CUDA(cudaGetLastError());
+  B200_CUDA(launch_chained(k_grouped_plan_kernel, 1, 1024, 0, stream, sizes, sizes_is_i64, gs, ge, num_groups, scratch));
   return 0;
 }
 

@@ -217,6 +217,7 @@ gated_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ C
   else __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_holder;
+  chain_wait();
 
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
@@ -591,19 +592,8 @@ static int launch_gated(const GatedMaps& t, const GatedArgs& p, int ctas, cudaSt
     ctas &= ~1;
   }
   B200_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kDynamicBytes));
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ctas, 1, 1);
-  cfg.blockDim = dim3(kNumThreads, 1, 1);
-  cfg.dynamicSmemBytes = L::kDynamicBytes;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = kPair ? 2 : 1;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  B200_CUDA(cudaLaunchKernelEx(&cfg, kern, t.a, t.b, t.h, t.gu, t.dgu, p));
+  B200_CUDA(launch_chained_clusters(kern, ctas, kNumThreads, L::kDynamicBytes, kPair ? 2 : 1, stream, t.a, t.b, t.h, t.gu,
+                                    t.dgu, p));
   return 0;
 }
 

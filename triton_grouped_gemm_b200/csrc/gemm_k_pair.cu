@@ -111,6 +111,7 @@ k_grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_con
   cluster_sync_all();  // both CTAs' barriers exist before anyone signals across the pair
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_holder;
+  chain_wait();
 
   const int* plan_starts = scratch + kPlanHeaderWords;
   const int* plan_tokens = plan_starts + num_groups;
@@ -431,10 +432,8 @@ int launch_k_grouped_pair(const CUtensorMap& tm_a, const CUtensorMap& tm_b, cons
   int grid = resident[dev];
   if (want_ctas > 0 && (want_ctas & ~1) < grid) grid = want_ctas & ~1;
   if (grid < 2) return set_error(kErrUnsupported, "the CTA-pair kernel needs at least 2 SMs");
-  kern<<<grid, kNumThreads, KPairSmem::kDynamicBytes, stream>>>(tm_a, tm_b, tm_c, c, num_groups, m_dim, n_dim, in_fmt,
-                                                                out_fp16, a_scale, b_scale, scratch,
-                                                                device_status_ptr());
-  B200_CUDA(cudaGetLastError());
+  B200_CUDA(launch_chained(kern, grid, kNumThreads, KPairSmem::kDynamicBytes, stream, tm_a, tm_b, tm_c, c, num_groups,
+                           m_dim, n_dim, in_fmt, out_fp16, a_scale, b_scale, scratch, device_status_ptr()));
   return 0;
 }
 

@@ -92,6 +92,7 @@ m_grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_con
   cluster_sync_all();  // both CTAs' barriers exist before anyone signals across the pair
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_holder;
+  chain_wait();
 
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer (both CTAs)
@@ -278,10 +279,9 @@ int launch_m_grouped_pair(const CUtensorMap& tm_a, const CUtensorMap& tm_b, cons
   int grid = cached_grid[dev];
   if (want_ctas > 0 && (want_ctas & ~1) < grid) grid = want_ctas & ~1;
   if (grid < 2) return set_error(kErrUnsupported, "the CTA-pair kernel needs at least 2 SMs");
-  kern<<<grid, kNumThreads, PairSmem::kDynamicBytes, stream>>>(tm_a, tm_b, tm_c, c, sizes, sizes_is_i64, num_groups,
-                                                               masked_stride, m_rows, n, k, in_fmt, out_fp16, a_scale,
-                                                               b_scale, device_status_ptr());
-  B200_CUDA(cudaGetLastError());
+  B200_CUDA(launch_chained(kern, grid, kNumThreads, PairSmem::kDynamicBytes, stream, tm_a, tm_b, tm_c, c, sizes,
+                           sizes_is_i64, num_groups, masked_stride, m_rows, n, k, in_fmt, out_fp16, a_scale, b_scale,
+                           device_status_ptr()));
   return 0;
 }
 

@@ -108,6 +108,7 @@ permute_rows_kernel(const uint4* __restrict__ x, const long long* __restrict__ p
                     long long units, unsigned* status) {
   constexpr int kStep = UnitWalk<kSpread>::kStep;
   const UnitWalk<kSpread> w;
+  chain_wait();
   for (long long u = w.first; u < units; u += w.stride) {
     if (u < tokens) {
       const long long mine = owned_row(pos, order, u, top_k, num_rows, w.lane, status);
@@ -145,6 +146,7 @@ combine_rows_kernel(const uint4* __restrict__ rows, const long long* __restrict_
                     long long tokens, int top_k, int row_vecs, long long num_rows, unsigned* status) {
   constexpr int kStep = UnitWalk<kSpread>::kStep;
   const UnitWalk<kSpread> w;
+  chain_wait();
   for (long long t = w.first; t < tokens; t += w.stride) {
     const long long mine = owned_row(pos, order, t, top_k, num_rows, w.lane, status);
     const float my_weight = w.lane < top_k ? (weights ? weights[t * top_k + w.lane] : 1.f) : 0.f;
@@ -206,6 +208,7 @@ combine_rows_grad_kernel(const uint4* __restrict__ dout, const uint4* __restrict
   constexpr int kWarps = kRowsThreads / 32;
   __shared__ float part[kWarps][kK];
   const UnitWalk<kSpread> w;
+  chain_wait();
   for (long long u = w.first; u < units; u += w.stride) {
     if (u < tokens) {
       const long long mine = owned_row(pos, order, u, top_k, num_rows, w.lane, status);
@@ -324,15 +327,14 @@ static int permute_rows(const void* x, const int64_t* pos, const int64_t* order,
   const long long units = tokens > row_units ? tokens : row_units;
   const RowsLaunch l = rows_launch(units, sms);
   auto kern = l.spread ? permute_rows_kernel<true> : permute_rows_kernel<false>;
-  kern<<<l.grid, kRowsThreads, 0, stream>>>(static_cast<const uint4*>(x), reinterpret_cast<const long long*>(pos),
-                                            reinterpret_cast<const long long*>(order), static_cast<uint4*>(out), tokens,
-                                            top_k, hidden / 8, num_rows, units, device_status_ptr());
-  B200_CUDA(cudaGetLastError());
+  B200_CUDA(launch_chained(kern, l.grid, kRowsThreads, 0, stream, static_cast<const uint4*>(x),
+                           reinterpret_cast<const long long*>(pos), reinterpret_cast<const long long*>(order),
+                           static_cast<uint4*>(out), tokens, top_k, hidden / 8, num_rows, units, device_status_ptr()));
   return 0;
 }
 
 template <bool kSpread, bool kFp16>
-static void launch_combine(int top_k, unsigned grid, cudaStream_t stream, const uint4* rows, const long long* pos,
+static cudaError_t launch_combine(int top_k, unsigned grid, cudaStream_t stream, const uint4* rows, const long long* pos,
                            const long long* order, const float* weights, uint4* out, long long tokens, int row_vecs,
                            long long num_rows) {
   auto kern = top_k == 1   ? combine_rows_kernel<kSpread, 1, 4, false, kFp16>
@@ -340,8 +342,8 @@ static void launch_combine(int top_k, unsigned grid, cudaStream_t stream, const 
               : top_k <= 4 ? combine_rows_kernel<kSpread, 4, 2, false, kFp16>
               : top_k <= 8 ? combine_rows_kernel<kSpread, 8, 1, false, kFp16>
                            : combine_rows_kernel<kSpread, 8, 1, true, kFp16>;
-  kern<<<grid, kRowsThreads, 0, stream>>>(rows, pos, order, weights, out, tokens, top_k, row_vecs, num_rows,
-                                          device_status_ptr());
+  return launch_chained(kern, grid, kRowsThreads, 0, stream, rows, pos, order, weights, out, tokens, top_k, row_vecs,
+                        num_rows, device_status_ptr());
 }
 
 static int combine_rows(const void* rows, const int64_t* pos, const int64_t* order, const float* weights, void* out,
@@ -356,22 +358,21 @@ static int combine_rows(const void* rows, const int64_t* pos, const int64_t* ord
   const RowsLaunch l = rows_launch(tokens, sms);
   auto go = l.spread ? (dtype ? launch_combine<true, true> : launch_combine<true, false>)
                      : (dtype ? launch_combine<false, true> : launch_combine<false, false>);
-  go(top_k, l.grid, stream, static_cast<const uint4*>(rows), reinterpret_cast<const long long*>(pos),
-     reinterpret_cast<const long long*>(order), weights, static_cast<uint4*>(out), tokens, hidden / 8, num_rows);
-  B200_CUDA(cudaGetLastError());
+  B200_CUDA(go(top_k, l.grid, stream, static_cast<const uint4*>(rows), reinterpret_cast<const long long*>(pos),
+               reinterpret_cast<const long long*>(order), weights, static_cast<uint4*>(out), tokens, hidden / 8, num_rows));
   return 0;
 }
 
 template <bool kSpread, bool kFp16>
-static void launch_combine_grad(int top_k, unsigned grid, cudaStream_t stream, const uint4* dout, const uint4* rows,
+static cudaError_t launch_combine_grad(int top_k, unsigned grid, cudaStream_t stream, const uint4* dout, const uint4* rows,
                                 const long long* pos, const long long* order, const float* weights, uint4* drows,
                                 float* dweights, long long tokens, int row_vecs, long long num_rows, long long units) {
   auto kern = top_k == 1   ? combine_rows_grad_kernel<kSpread, 1, kFp16>
               : top_k == 2 ? combine_rows_grad_kernel<kSpread, 2, kFp16>
               : top_k <= 4 ? combine_rows_grad_kernel<kSpread, 4, kFp16>
                            : combine_rows_grad_kernel<kSpread, 8, kFp16>;
-  kern<<<grid, kRowsThreads, 0, stream>>>(dout, rows, pos, order, weights, drows, dweights, tokens, top_k, row_vecs,
-                                          num_rows, units, device_status_ptr());
+  return launch_chained(kern, grid, kRowsThreads, 0, stream, dout, rows, pos, order, weights, drows, dweights, tokens,
+                        top_k, row_vecs, num_rows, units, device_status_ptr());
 }
 
 static int combine_rows_grad(const void* dout, const void* rows, const int64_t* pos, const int64_t* order,
@@ -391,10 +392,9 @@ static int combine_rows_grad(const void* dout, const void* rows, const int64_t* 
   const RowsLaunch l = rows_launch(units, sms);
   auto go = l.spread ? (dtype ? launch_combine_grad<true, true> : launch_combine_grad<true, false>)
                      : (dtype ? launch_combine_grad<false, true> : launch_combine_grad<false, false>);
-  go(top_k, l.grid, stream, static_cast<const uint4*>(dout), static_cast<const uint4*>(rows),
-     reinterpret_cast<const long long*>(pos), reinterpret_cast<const long long*>(order), weights,
-     static_cast<uint4*>(drows), dweights, tokens, hidden / 8, num_rows, units);
-  B200_CUDA(cudaGetLastError());
+  B200_CUDA(go(top_k, l.grid, stream, static_cast<const uint4*>(dout), static_cast<const uint4*>(rows),
+               reinterpret_cast<const long long*>(pos), reinterpret_cast<const long long*>(order), weights,
+               static_cast<uint4*>(drows), dweights, tokens, hidden / 8, num_rows, units));
   return 0;
 }
 

@@ -404,4 +404,11 @@ __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// Programmatic dependent launch: a kernel that launch_chained() queued may start before its predecessor in the stream has
+// ended.  chain_wait() comes before its first access to global memory and returns once the predecessor has ended and its
+// writes can be seen; every thread calls it, so the kernel cannot end before its predecessor either.  It does nothing
+// after an ordinary launch.  A predecessor's blocks let the successor start when they leave, or with chain_release().
+__device__ __forceinline__ void chain_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void chain_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 }  // namespace b200
