@@ -302,3 +302,20 @@ def test_captured_forward_and_backward_replay():
         eager = _run(x2, w13, w2, new_sizes, "silu", dy2)
         assert all(torch.equal(a, b) for a, b in zip(captured, eager))
     assert _lib.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_full_and_partial_tiles_in_turn(dtype):
+    """Every block of the launch gets a full tile, then a group's last one whose rows end inside one of its warps, then a
+    full one again: what a warp stages for the third may not overtake the first one's store."""
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    sizes = ([128 * sms] + [(20, 52, 84, 116)[i % 4] for i in range(sms)]) * 3
+    x, w13, w2, dy = _inputs(sizes, 16, 64, 0, dtype)
+    want = _run(x, w13, w2, sizes, "silu", dy)
+    _check(want, block(x, w13, w2, sizes, "silu", dy))
+    group_sizes = torch.tensor(sizes, device=DEV)
+    for _ in range(30):
+        with torch.no_grad():
+            assert torch.equal(grouped_gated_ffn(x, w13, w2, group_sizes), want[0])
+        for value, first in zip(_run(x, w13, w2, sizes, "silu", dy), want):
+            assert torch.equal(value, first)

@@ -397,7 +397,7 @@ gated_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ C
             uint8_t* buf_h = epi + (sel & (L::kEpiBuffers - 1)) * 4096;
             uint8_t* buf_g = epi + ((sel + 1) & (L::kEpiBuffers - 1)) * 4096;
             uint8_t* buf_u = epi + ((sel + 2) & (L::kEpiBuffers - 1)) * 4096;
-            sel += kSave ? 3 : 1;
+            if (full) sel += kSave ? 3 : 1;   // only with a store: the wait above counts stores
 #pragma unroll 1
             for (int s = 0; s < 2; ++s) {
               uint32_t g[32], u[32];
