@@ -108,6 +108,8 @@ int b200gemm_m_grouped_masked(const void* lhs, const void* rhs, void* out, const
  *   A [k_total, m_dim], B [k_total, n_dim] row-major; C [G, m_dim, n_dim].
  *   Token ranges: group_start/group_end (int32 [G], both or neither) if given, else the
  *   running prefix of sizes [G].  Requires m_dim % 8 == 0, n_dim % 8 == 0.
+ *   A group that reaches past row k_total is cut off there and B200GEMM_DEV_BAD_GROUP_SIZE is set; negative
+ *   sizes count as zero.
  *   workspace: optional device scratch of b200gemm_k_grouped_workspace_bytes(G) bytes (contents
  *   need no initialisation).  With it, tiles are claimed dynamically, groups with the most
  *   tokens first (tile cost varies with the group's token count); NULL = fixed round-robin

@@ -28,6 +28,7 @@
 #include "../../include/b200gemm.h"
 #include "common.cuh"
 #include "gemm_tile.cuh"
+#include "token_range.cuh"
 
 namespace b200 {
 
@@ -45,39 +46,43 @@ struct KGroupedSmem {
 };
 
 // Token range of a group: either explicit int32 [start, end) arrays, or a running exclusive
-// prefix over the group sizes (`g` only moves forward).
+// prefix over the group sizes (`g` only moves forward).  Both are cut off at k_total, like the groups of the M-grouped
+// kernels at their rows; the cut is remembered in `cut`.
 struct TokenRange {
   const void* sizes;
   const int* starts;
   const int* ends;
   int sizes_i64;
   int cur;
+  bool cut;
+  long long total;
   long long start;
-  __device__ __forceinline__ long long size_of(int i) const {
-    long long v = sizes_i64 ? static_cast<const long long*>(sizes)[i]
-                            : static_cast<long long>(static_cast<const int*>(sizes)[i]);
-    return v < 0 ? 0 : v;
+  __device__ __forceinline__ TokenSpan span(int i) const {
+    if (starts) return span_of_bounds(starts[i], ends[i], total);
+    return span_of_size(start, sizes_i64 ? static_cast<const long long*>(sizes)[i]
+                                         : static_cast<long long>(static_cast<const int*>(sizes)[i]), total);
   }
-  __device__ __forceinline__ void init(const void* s, int i64, const int* gs, const int* ge) {
+  __device__ __forceinline__ void init(const void* s, int i64, const int* gs, const int* ge, long long k_total) {
     sizes = s;
     sizes_i64 = i64;
     starts = gs;
     ends = ge;
     cur = 0;
+    cut = false;
+    total = k_total;
     start = 0;
   }
   // returns the number of tokens of group g; start = first token row of g
   __device__ __forceinline__ long long seek(int g) {
-    if (starts) {
-      start = starts[g];
-      const long long t = static_cast<long long>(ends[g]) - start;
-      return t < 0 ? 0 : t;
+    while (!starts && cur < g) {
+      const TokenSpan s = span(cur++);
+      start += s.tokens;
+      cut |= s.cut;
     }
-    while (cur < g) {
-      start += size_of(cur);
-      ++cur;
-    }
-    return size_of(g);
+    const TokenSpan s = span(g);
+    start = s.start;
+    cut |= s.cut;
+    return s.tokens;
   }
 };
 
@@ -89,27 +94,22 @@ __host__ __device__ inline long long k_grouped_scratch_words(int num_groups) {
 __global__ void __launch_bounds__(1024) k_grouped_plan_kernel(const void* __restrict__ sizes, int sizes_i64,
                                                               const int* __restrict__ group_start,
                                                               const int* __restrict__ group_end, int num_groups,
-                                                              int* __restrict__ scratch) {
+                                                              long long k_total, int* __restrict__ scratch,
+                                                              unsigned* status) {
   chain_wait();
   chain_release();
   int* starts = scratch + kPlanHeaderWords;
   int* tokens = starts + num_groups;
   int* order = tokens + num_groups;
-  auto size_of = [&](int g) -> long long {
-    long long v;
-    if (group_start) v = static_cast<long long>(group_end[g]) - group_start[g];
-    else v = sizes_i64 ? static_cast<const long long*>(sizes)[g] : static_cast<long long>(static_cast<const int*>(sizes)[g]);
-    return v < 0 ? 0 : v;
-  };
   if (threadIdx.x == 0) {
     scratch[0] = 0;  // tile counter
-    long long run = 0;
+    TokenRange range;
+    range.init(sizes, sizes_i64, group_start, group_end, k_total);
     for (int g = 0; g < num_groups; ++g) {  // G is small (<= 4096): a serial prefix is a few microseconds
-      const long long t = size_of(g);
-      starts[g] = group_start ? group_start[g] : static_cast<int>(run);
-      tokens[g] = static_cast<int>(t);
-      run += t;
+      tokens[g] = static_cast<int>(range.seek(g));   // both fit: start + tokens <= k_total < 2^31
+      starts[g] = static_cast<int>(range.start);
     }
+    if (range.cut && status) atomicOr(status, kDevBadGroupSize);
   }
   __syncthreads();
   // rank of every group in the order "more tokens first, ties by index" (stable)
@@ -238,7 +238,7 @@ k_grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
     TokenRange tr;
-    tr.init(sizes, sizes_i64, group_start, group_end);
+    tr.init(sizes, sizes_i64, group_start, group_end, k_total);
     int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
@@ -329,10 +329,11 @@ k_grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
         }
       }
     }
+    if (!kBalanced && tr.cut && lane == 0 && status) atomicOr(status, kDevBadGroupSize);
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
     TokenRange tr;
-    tr.init(sizes, sizes_i64, group_start, group_end);
+    tr.init(sizes, sizes_i64, group_start, group_end, k_total);
     const uint32_t a_fmt = kFp8 ? static_cast<uint32_t>(in_fmt & 0xF) : static_cast<uint32_t>(in_fmt);
     const uint32_t b_fmt = kFp8 ? static_cast<uint32_t>((in_fmt >> 4) & 0xF) : static_cast<uint32_t>(in_fmt);
     const uint32_t mn_major = kFp8 ? 0u : 1u;
@@ -405,7 +406,7 @@ k_grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
   } else {
     // ------------------------------------------------------------ epilogue (warps 2..5)
     TokenRange tr;
-    tr.init(sizes, sizes_i64, group_start, group_end);
+    tr.init(sizes, sizes_i64, group_start, group_end, k_total);
     const int quarter = warp & 3;
     uint8_t* epi_stage = smem + L::kEpiOffset + quarter * kEpiStageBytesPerWarp;
     int epi_sel = 0;
@@ -473,7 +474,8 @@ static int launch_k_grouped(const CUtensorMap& tm_a, const CUtensorMap& tm_b, co
     // balanced: plan (starts, token counts, longest-first order, zeroed tile counter), then the GEMM
     auto kern = k_grouped_kernel<kBlockN, kStages, kFp8, true>;
     B200_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kDynamicBytes));
-    B200_CUDA(launch_chained(k_grouped_plan_kernel, 1, 1024, 0, stream, sizes, sizes_is_i64, gs, ge, num_groups, scratch));
+    B200_CUDA(launch_chained(k_grouped_plan_kernel, 1, 1024, 0, stream, sizes, sizes_is_i64, gs, ge, num_groups, k_total,
+                             scratch, status));
     B200_CUDA(launch_chained(kern, grid, kNumThreads, L::kDynamicBytes, stream, tm_a, tm_b, tm_c, c, sizes, sizes_is_i64, gs,
                              ge, num_groups, m_dim, n_dim, k_total, in_fmt, out_fp16, a_scale, b_scale, scratch, status));
   } else {
@@ -510,19 +512,20 @@ static bool want_k_pair(const int* scratch, int num_groups, int m_dim, int n_dim
   return m_dim >= 256 && n_dim >= 256 && tiles >= grid;
 }
 
-static int launch_plan(const void* sizes, int sizes_is_i64, const int* gs, const int* ge, int num_groups, int* scratch,
-                       cudaStream_t stream) {
-  B200_CUDA(launch_chained(k_grouped_plan_kernel, 1, 1024, 0, stream, sizes, sizes_is_i64, gs, ge, num_groups, scratch));
+static int launch_plan(const void* sizes, int sizes_is_i64, const int* gs, const int* ge, int num_groups, long long k_total,
+                       int* scratch, cudaStream_t stream) {
+  B200_CUDA(launch_chained(k_grouped_plan_kernel, 1, 1024, 0, stream, sizes, sizes_is_i64, gs, ge, num_groups, k_total,
+                           scratch, device_status_ptr()));
   return 0;
 }
 
 // for the other K-grouped translation units: validate a workspace and queue the plan kernel
 // (starts, token counts, longest-first order) on it; *out = nullptr when no workspace was given
 int k_grouped_plan_into(void* workspace, long long workspace_bytes, const void* sizes, int sizes_is_i64,
-                        int num_groups, const char* who, int** out, cudaStream_t stream) {
+                        int num_groups, long long k_total, const char* who, int** out, cudaStream_t stream) {
   int rc = check_scratch(workspace, workspace_bytes, num_groups, who, out);
   if (rc || !*out) return rc;
-  return launch_plan(sizes, sizes_is_i64, nullptr, nullptr, num_groups, *out, stream);
+  return launch_plan(sizes, sizes_is_i64, nullptr, nullptr, num_groups, k_total, *out, stream);
 }
 
 // tile width: 256 output columns unless that leaves SMs without a tile
@@ -593,7 +596,7 @@ static int k_grouped_bf16(const void* a, const void* b, void* c, const void* siz
   }
   const int in_fmt = dtype == 1 ? 0 : 1;  // UMMA kind::f16 operand format: 0 = f16, 1 = bf16
   if (want_k_pair(scratch, num_groups, m_dim, n_dim, grid)) {
-    int rc = launch_plan(sizes, sizes_is_i64, group_start, group_end, num_groups, scratch, stream);
+    int rc = launch_plan(sizes, sizes_is_i64, group_start, group_end, num_groups, k_total, scratch, stream);
     if (rc) return rc;
     return launch_k_grouped_pair<false>(tm_a, tm_b, tm_c, c, num_groups, m_dim, n_dim, in_fmt, dtype, nullptr, nullptr,
                                         scratch, grid, stream);
@@ -678,7 +681,7 @@ extern "C" int b200gemm_fp8_k_grouped_rowcol(const void* x, const float* x_scale
   }
   const int in_fmt = fmt_x | (fmt_y << 4);
   if (pair) {
-    int rc = launch_plan(tokens_per_expert, sizes_is_i64, nullptr, nullptr, num_groups, scratch, stream);
+    int rc = launch_plan(tokens_per_expert, sizes_is_i64, nullptr, nullptr, num_groups, k_total, scratch, stream);
     if (rc) return rc;
     return launch_k_grouped_pair<true>(tm_x, tm_y, tm_c, out, num_groups, m_dim, n_dim, in_fmt, /*out bf16*/ 0, x_scale,
                                        y_scale, scratch, grid, stream);

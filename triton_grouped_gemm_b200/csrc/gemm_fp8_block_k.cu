@@ -514,7 +514,8 @@ int b200gemm_fp8_k_grouped_block(const void* x8, const float* x_scale, const voi
   const long long kb_total = m_expand / 128;
   int* plan = nullptr;
   {
-    int rc = k_grouped_plan_into(workspace, workspace_bytes, padded_sizes, sizes_is_i64, num_groups, who, &plan, stream);
+    int rc = k_grouped_plan_into(workspace, workspace_bytes, padded_sizes, sizes_is_i64, num_groups, m_expand, who, &plan,
+                                 stream);
     if (rc) return rc;
   }
   if (pair)
