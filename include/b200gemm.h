@@ -147,8 +147,9 @@ int b200gemm_k_grouped_static_scratch(const void* a, const void* b, void* c, con
  * accumulate, one rounding.  a [m_rows, k]; w13 [G, 2 inter, k]: gate rows, then up rows.
  *   saved, saved_exps: NULL (inference), or both: g and u are kept for the gradient - saved
  *   [m_rows, 2 inter] 16-bit codes and saved_exps, b200gemm_gated_exponent_bytes(m_rows, inter) bytes
- *   (one power of two per 32 columns; the format is the library's own).  A value of g or u that is not
- *   finite reads back as NaN.
+ *   (one power of two per 32 columns; the format is the library's own).  A kept value is off by at most 2^-11 of
+ *   itself while it is above 2^-28 of the largest of its 32 (fp16: above 2^-12, and by 2^-23 of it below).  NaN reads
+ *   back as NaN, an infinity as itself (fp16: as NaN).
  *   masked_stride > 0: masked row layout (rows g * stride ..., sizes[g] valid); 0: compact rows.
  *   tail, tail_cols: NULL, or a [m_rows, tail_cols] 16-bit matrix (another buffer than the operands)
  *   whose rows behind the last group are set to zero; compact rows only.

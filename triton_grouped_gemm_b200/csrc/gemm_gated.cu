@@ -14,7 +14,8 @@
 //     the row (see below).  That block is what a thread holds in registers, so its maximum costs no exchange, and what
 //     the gradients lose is the rounding of dg and du alone, which the tensor cores ask for: error of dx in 2-norm,
 //     4096 rows, K 2048, I 768: bf16 layers 2.4e-3, and 3.0e-3 with g and u in bf16 (1.7e-3 is the rounding of dx
-//     itself); fp16 layers 2.9e-4 and 3.8e-4 (2.1e-4).
+//     itself); fp16 layers 3.0e-4 and 3.8e-4 (2.1e-4).  A column of fp16 layers far below its neighbours keeps the accuracy
+//     that plain fp16 would give it down to 2^-12 of the largest of them, and loses a bit with every further factor of two.
 //   * Everything else is the M-grouped kernel's: persistent CTAs, one walk over the group sizes, TMA ring, one MMA
 //     issuer, two accumulators, epilogue warps that store through swizzled staging buffers.
 //
@@ -22,7 +23,8 @@
 // the same GPU: forward 2.78 ms (2.72), keeping g and u 3.26 ms (3.38 - the same, both at the power limit), gradient
 // 1.94 ms (1.66; it reads 2.0 GB and writes 2.0 GB where the plain product writes 1.0 GB).  With integer arithmetic for
 // the codes and an exactly rounded reciprocal they took 3.96 and 3.54 ms: the epilogue, not the tensor cores, was the
-// bound.  With 128 rows over 80 of 128 groups the forward is bound by the weights: 503 MB in 89 us, 5.65 TB/s.
+// bound, and it still is in fp16 layers: keeping g and u 3.8-4.2 ms, gradient 2.2-2.5 ms (gelu 4.0 and 2.7; bf16 layers
+// in the same runs 3.0 and 1.9, gelu 3.5 and 2.1).  With 128 rows over 80 of 128 groups the forward is bound by the weights: 503 MB in 89 us, 5.65 TB/s.
 //
 // Rows behind the last group have no product; the epilogue warps zero them in `tail` (the layer's output in the
 // forward call, its input gradient in the backward call) once their tiles are done.
@@ -35,6 +37,7 @@
 #include "activation.cuh"
 #include "common.cuh"
 #include "gemm_tile.cuh"
+#include "kept_code.cuh"
 
 namespace b200 {
 
@@ -44,15 +47,11 @@ enum class GatedMode { kForward, kForwardSave, kBackward };
 // A block of 32 values v is kept as 16-bit codes and the fp32 exponent field e of its largest finite magnitude.
 //   bf16 layers   code = fp16(v * 2^(141 - e)): the largest lies in [2^14, 2^15), 10 mantissa bits down to 2^-28 of it.
 //                 One multiplication and half a conversion per value, and fp16's own infinities and NaN.
-//   fp16 layers   fp16 would add as much error as the output's rounding, so one exponent bit more is given to the
-//                 mantissa twice over: v is scaled until the largest has exponent field kTop, rounded to 12 bits in
-//                 integer arithmetic, and the 5 upper exponent bits, then zero, are dropped: 1 sign, 3 exponent, 12
-//                 mantissa bits, even steps of 2^-17 of the largest's power of two below 2^-5 of it.  The all-ones
-//                 code stands for a value that was not finite and reads back as NaN.
+//   fp16 layers   fp16 would add as much error as the output's rounding, so the values near the largest get two mantissa
+//                 bits more, which are taken from the exponents far below it (kept_code.cuh).  Integer arithmetic, 1.5 and
+//                 2 instructions per value more than with the same mantissa for all: 4 096 rows over 8 groups, K 2048,
+//                 I 768, silu, keeping g and u 35.5 -> 36.3 us, gradient 29.8 -> 30.2 us.
 constexpr uint32_t kBlockExpMin = 15;   // keeps 2^(141 - e) and its inverse normal numbers
-constexpr int kCodeMant = 12;
-constexpr int kCodeDrop = 23 - kCodeMant;
-constexpr uint32_t kCodeTop = 6;        // one below all ones (7): rounding may carry into the exponent
 
 __device__ __forceinline__ uint32_t block_exponent(const uint32_t (&v)[32]) {
   float m = 0.f;
@@ -77,18 +76,16 @@ __device__ __forceinline__ float block_up(uint32_t e) {
   return __uint_as_float((kFp16 ? e : e - 14u) << 23);
 }
 
-__device__ __forceinline__ uint32_t code12(uint32_t v, float down) {
-  // times 2^-135 (a denormal): [2^14, 2^15) -> [2^-121, 2^-120), whose exponent field is kCodeTop
-  const uint32_t f = __float_as_uint(__uint_as_float(v) * down * __uint_as_float(1u << 14));
-  const uint32_t mag = f & 0x7FFFFFFFu;
-  const uint32_t code = (mag + ((1u << (kCodeDrop - 1)) - 1) + ((mag >> kCodeDrop) & 1u)) >> kCodeDrop;
-  return min(code, 0x7FFFu) | ((f >> 16) & 0x8000u);
+__device__ __forceinline__ uint32_t code16(uint32_t v, float down) {
+  // times 2^-128 (a denormal): [2^14, 2^15) -> [2^-114, 2^-113), whose exponent field is kKeptTop
+  const uint32_t f = __float_as_uint(__uint_as_float(v) * down * __uint_as_float(1u << 21));
+  return kept_code(f & 0x7FFFFFFFu) | ((f >> 16) & 0x8000u);
 }
 
 template <bool kFp16>
 __device__ __forceinline__ uint32_t encode2(uint32_t lo, uint32_t hi, float down) {
   if constexpr (!kFp16) return pack2_16bit(__uint_as_float(lo) * down, __uint_as_float(hi) * down, 1);
-  return code12(lo, down) | code12(hi, down) << 16;
+  return code16(lo, down) | code16(hi, down) << 16;
 }
 
 template <bool kFp16>
@@ -97,12 +94,14 @@ __device__ __forceinline__ float2 decode2(uint32_t codes, float up) {
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&codes));
     return make_float2(f.x * up, f.y * up);
   }
-  auto one = [&](uint32_t code) {
-    const uint32_t mag = code & 0x7FFFu;
-    const float f = __uint_as_float((mag << kCodeDrop) | ((code & 0x8000u) << 16)) * __uint_as_float((127u + 127u - kCodeTop) << 23) * up;
-    return mag == 0x7FFFu ? __uint_as_float(0x7FFFFFFFu) : f;
+  const uint32_t mags = codes & 0x7FFF7FFFu;
+  const uint32_t bits = kept_bits2(mags, [](uint32_t a, uint32_t b) { return __vminu2(a, b); });
+  auto one = [&](uint32_t magnitude, uint32_t sign, bool finite) {
+    const float f = __uint_as_float(magnitude | (sign & 0x80000000u)) * __uint_as_float((127u + 127u - kKeptTop) << 23) * up;
+    return finite ? f : __uint_as_float(0x7FFFFFFFu);
   };
-  return make_float2(one(codes & 0xFFFFu), one(codes >> 16));
+  return make_float2(one((bits << 11) & 0x07FFF800u, codes << 16, (mags & 0xFFFFu) != 0x7FFFu),
+                     one((bits >> 5) & 0x07FFF800u, codes, mags < 0x7FFF0000u));
 }
 
 // runs f with the activation as a compile-time constant
