@@ -86,6 +86,8 @@ struct TokenRange {
   }
 };
 
+constexpr int kMaxBalancedGroups = 4096;
+
 // Scratch layout (int32 words): [0] tile counter, [1..63] unused, then starts[G], tokens[G], order[G].
 __host__ __device__ inline long long k_grouped_scratch_words(int num_groups) {
   return kPlanHeaderWords + 3ll * num_groups;
@@ -101,16 +103,42 @@ __global__ void __launch_bounds__(1024) k_grouped_plan_kernel(const void* __rest
   int* starts = scratch + kPlanHeaderWords;
   int* tokens = starts + num_groups;
   int* order = tokens + num_groups;
-  if (threadIdx.x == 0) {
-    scratch[0] = 0;  // tile counter
-    TokenRange range;
-    range.init(sizes, sizes_i64, group_start, group_end, k_total);
-    for (int g = 0; g < num_groups; ++g) {  // G is small (<= 4096): a serial prefix is a few microseconds
-      tokens[g] = static_cast<int>(range.seek(g));   // both fit: start + tokens <= k_total < 2^31
-      starts[g] = static_cast<int>(range.start);
-    }
-    if (range.cut && status) atomicOr(status, kDevBadGroupSize);
+  __shared__ unsigned rows[kMaxBalancedGroups];   // tokens of every group, cut to k_total (< 2^31)
+  bool cut = false;
+  for (int g = threadIdx.x; g < num_groups; g += blockDim.x) {
+    const TokenSpan s = group_start ? span_of_bounds(group_start[g], group_end[g], k_total)
+                                    : span_of_size(0, sizes_i64 ? static_cast<const long long*>(sizes)[g]
+                                                                : static_cast<long long>(static_cast<const int*>(sizes)[g]), k_total);
+    rows[g] = static_cast<unsigned>(s.tokens);
+    if (group_start) starts[g] = static_cast<int>(s.start);
+    cut |= s.cut;
   }
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    // Sums over the groups before, 32 groups at a time.  They saturate at k_total, which is what a walk from group to group
+    // gives where every group is cut off there, whatever order they are formed in.
+    const unsigned total = static_cast<unsigned>(k_total);
+    unsigned run = 0;
+    if (threadIdx.x == 0) scratch[0] = 0;  // tile counter
+    for (int g = threadIdx.x; g - static_cast<int>(threadIdx.x) < num_groups; g += 32) {
+      unsigned mine = g < num_groups ? rows[g] : 0u, upto = mine;
+      if (!group_start) {
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const unsigned up = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+          if (threadIdx.x >= o) upto = min(upto + up, total);
+        }
+        const unsigned up = __shfl_up_sync(0xFFFFFFFFu, upto, 1);
+        const unsigned start = min(run + (threadIdx.x ? up : 0u), total);
+        run = min(run + __shfl_sync(0xFFFFFFFFu, upto, 31), total);
+        cut |= mine > total - start;
+        mine = min(mine, total - start);
+        if (g < num_groups) starts[g] = static_cast<int>(start);
+      }
+      if (g < num_groups) tokens[g] = static_cast<int>(mine);
+    }
+  }
+  if (cut && status) atomicOr(status, kDevBadGroupSize);
   __syncthreads();
   // rank of every group in the order "more tokens first, ties by index" (stable)
   for (int g = threadIdx.x; g < num_groups; g += blockDim.x) {
@@ -486,8 +514,6 @@ static int launch_k_grouped(const CUtensorMap& tm_a, const CUtensorMap& tm_b, co
   }
   return 0;
 }
-
-constexpr int kMaxBalancedGroups = 4096;
 
 // validates a caller-provided scratch buffer for the balanced scheduler; nullptr = round-robin
 static int check_scratch(void* workspace, long long workspace_bytes, int num_groups, const char* who, int** out) {
