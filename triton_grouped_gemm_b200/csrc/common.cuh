@@ -10,6 +10,7 @@
 #include <stdio.h>
 
 #include "ptx.cuh"
+#include "bounded_wait.cuh"
 
 namespace b200 {
 
@@ -89,28 +90,15 @@ inline cudaError_t launch_chained(void (*kern)(Params...), unsigned grid, unsign
 // Every spin on an mbarrier gives up after kWaitLimitNs; the waiting role then raises the
 // CTA-wide abort flag, records which role timed out in the device status word and leaves
 // its loop, so a protocol error ends in an error code instead of a hung GPU.
-constexpr uint64_t kWaitLimitNs = 2000000000ull;  // 2 s
-
+// Called by all 32 lanes of a warp, which get one answer (bounded_wait.cuh).
 __device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t parity, volatile int* abort_flag,
                                              unsigned* status, unsigned role_bit) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const uint64_t t0 = global_timer_ns();
-  uint32_t spins = 0;
-  while (!mbar_try_wait(bar, parity)) {
-    if ((++spins & 63u) == 0u) {
-      if (*abort_flag) return false;
-      if (global_timer_ns() - t0 > kWaitLimitNs) {
-        *abort_flag = 1;
-        if (status) atomicOr(status, role_bit);
-        return false;
-      }
-    }
-  }
-  return true;
+  return wait_together<64>([&]() { return mbar_try_wait(bar, parity); }, abort_flag, status, role_bit);
 }
 
-// Same for a role that has nothing else to do and shares its scheduler with warps that compute: the hardware
-// parks the thread for up to 20 us per attempt instead of the default, so it issues next to nothing.
+// For a role that has nothing else to do and shares its scheduler with warps that compute: the hardware parks the
+// thread for up to 20 us per attempt instead of the default, so it issues next to nothing.  Lane by lane: callers vote on
+// the answer.
 __device__ __forceinline__ bool wait_bounded_parked(uint32_t bar, uint32_t parity, volatile int* abort_flag,
                                                     unsigned* status, unsigned role_bit) {
   uint64_t t0 = 0;
@@ -148,23 +136,10 @@ __device__ __forceinline__ bool wait_bounded_spin(uint32_t bar, uint32_t parity,
   return true;
 }
 
-// same, for barriers that the peer CTA of a pair arrives on (cluster-scope acquire)
+// wait_bounded() for barriers that the peer CTA of a pair arrives on (cluster-scope acquire)
 __device__ __forceinline__ bool wait_bounded_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag,
                                                      unsigned* status, unsigned role_bit) {
-  if (mbar_try_wait_cluster(bar, parity)) return true;
-  const uint64_t t0 = global_timer_ns();
-  uint32_t spins = 0;
-  while (!mbar_try_wait_cluster(bar, parity)) {
-    if ((++spins & 63u) == 0u) {
-      if (*abort_flag) return false;
-      if (global_timer_ns() - t0 > kWaitLimitNs) {
-        *abort_flag = 1;
-        if (status) atomicOr(status, role_bit);
-        return false;
-      }
-    }
-  }
-  return true;
+  return wait_together<64>([&]() { return mbar_try_wait_cluster(bar, parity); }, abort_flag, status, role_bit);
 }
 
 // ------------------------------------------------------------------ group walker
