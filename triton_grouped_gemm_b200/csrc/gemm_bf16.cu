@@ -41,9 +41,9 @@ struct MGroupedSmem {
 template <int kBlockN, int kStages, bool kBMnMajor, bool kFp8>
 __global__ void __launch_bounds__(kNumThreads, 1)
 m_grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
-                 const __grid_constant__ CUtensorMap tm_c, void* __restrict__ c_ptr, const void* __restrict__ sizes, int sizes_i64, int num_groups,
+                 const __grid_constant__ CUtensorMap tm_c, void* __restrict__ c_ptr, const void* sizes, int sizes_i64, int num_groups,
                  int masked_stride, long long m_rows, int n, int k, int in_fmt, int out_fp16,
-                 const float* __restrict__ a_scale, const float* __restrict__ b_scale, unsigned* status) {
+                 const float* a_scale, const float* b_scale, unsigned* status) {
   static_assert(!(kFp8 && kBMnMajor), "fp8 operands are K-major only");
   constexpr int kElemsPerKb = kFp8 ? 128 : 64;
   using L = MGroupedSmem<kBlockN, kStages>;
@@ -203,7 +203,7 @@ m_grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
       float rs = 1.0f;
       const float* cs = nullptr;
       if constexpr (kFp8) {
-        rs = row_ok ? __ldg(a_scale + row) : 0.f;
+        rs = row_ok ? a_scale[row] : 0.f;
         cs = b_scale + static_cast<long long>(w.g) * n;
       }
       if (warp_full)

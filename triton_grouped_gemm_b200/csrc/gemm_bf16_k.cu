@@ -45,6 +45,11 @@ struct KGroupedSmem {
   static constexpr int kDynamicBytes = kTotal + 1024;
 };
 
+__device__ __forceinline__ long long token_count(const void* sizes, int sizes_i64, int g) {
+  return sizes_i64 ? static_cast<const long long*>(sizes)[g]
+                   : static_cast<long long>(static_cast<const int*>(sizes)[g]);
+}
+
 // Token range of a group: either explicit int32 [start, end) arrays, or a running exclusive
 // prefix over the group sizes (`g` only moves forward).  Both are cut off at k_total, like the groups of the M-grouped
 // kernels at their rows; the cut is remembered in `cut`.
@@ -59,8 +64,7 @@ struct TokenRange {
   long long start;
   __device__ __forceinline__ TokenSpan span(int i) const {
     if (starts) return span_of_bounds(starts[i], ends[i], total);
-    return span_of_size(start, sizes_i64 ? static_cast<const long long*>(sizes)[i]
-                                         : static_cast<long long>(static_cast<const int*>(sizes)[i]), total);
+    return span_of_size(start, token_count(sizes, sizes_i64, i), total);
   }
   __device__ __forceinline__ void init(const void* s, int i64, const int* gs, const int* ge, long long k_total) {
     sizes = s;
@@ -93,11 +97,9 @@ __host__ __device__ inline long long k_grouped_scratch_words(int num_groups) {
   return kPlanHeaderWords + 3ll * num_groups;
 }
 
-__global__ void __launch_bounds__(1024) k_grouped_plan_kernel(const void* __restrict__ sizes, int sizes_i64,
-                                                              const int* __restrict__ group_start,
-                                                              const int* __restrict__ group_end, int num_groups,
-                                                              long long k_total, int* __restrict__ scratch,
-                                                              unsigned* status) {
+__global__ void __launch_bounds__(1024) k_grouped_plan_kernel(const void* sizes, int sizes_i64, const int* group_start,
+                                                              const int* group_end, int num_groups, long long k_total,
+                                                              int* scratch, unsigned* status) {
   chain_wait();
   chain_release();
   int* starts = scratch + kPlanHeaderWords;
@@ -107,8 +109,7 @@ __global__ void __launch_bounds__(1024) k_grouped_plan_kernel(const void* __rest
   bool cut = false;
   for (int g = threadIdx.x; g < num_groups; g += blockDim.x) {
     const TokenSpan s = group_start ? span_of_bounds(group_start[g], group_end[g], k_total)
-                                    : span_of_size(0, sizes_i64 ? static_cast<const long long*>(sizes)[g]
-                                                                : static_cast<long long>(static_cast<const int*>(sizes)[g]), k_total);
+                                    : span_of_size(0, token_count(sizes, sizes_i64, g), k_total);
     rows[g] = static_cast<unsigned>(s.tokens);
     if (group_start) starts[g] = static_cast<int>(s.start);
     cut |= s.cut;
@@ -161,10 +162,10 @@ __global__ void __launch_bounds__(1024) k_grouped_plan_kernel(const void* __rest
 template <int kBlockN, int kStages, bool kFp8, bool kBalanced>
 __global__ void __launch_bounds__(kNumThreads, 1)
 k_grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
-                 const __grid_constant__ CUtensorMap tm_c, void* __restrict__ c_ptr, const void* __restrict__ sizes, int sizes_i64,
-                 const int* __restrict__ group_start, const int* __restrict__ group_end, int num_groups, int m_dim,
-                 int n_dim, long long k_total, int in_fmt, int out_fp16, const float* __restrict__ a_scale,
-                 const float* __restrict__ b_scale, int* __restrict__ scratch, unsigned* status) {
+                 const __grid_constant__ CUtensorMap tm_c, void* __restrict__ c_ptr, const void* sizes, int sizes_i64,
+                 const int* group_start, const int* group_end, int num_groups, int m_dim,
+                 int n_dim, long long k_total, int in_fmt, int out_fp16, const float* a_scale,
+                 const float* b_scale, int* scratch, unsigned* status) {
   constexpr int kTokensPerKb = kFp8 ? 128 : kBlockK;
   using L = KGroupedSmem<kBlockN, kStages>;
   extern __shared__ uint8_t smem_raw[];
@@ -281,11 +282,11 @@ k_grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
       } else if (nx_step == 1) {
         nx_t = __shfl_sync(0xFFFFFFFFu, nx_t, 0);
         nx_slot = static_cast<int>(nx_t / tiles_per_group);
-        if (nx_t < num_tiles) asm volatile("ld.global.nc.s32 %0, [%1];" : "=r"(nx_g) : "l"(plan_order + nx_slot));
+        if (nx_t < num_tiles) asm volatile("ld.global.s32 %0, [%1];" : "=r"(nx_g) : "l"(plan_order + nx_slot));
       } else if (nx_step == 2) {
         if (nx_t < num_tiles) {
-          asm volatile("ld.global.nc.s32 %0, [%1];" : "=r"(nx_tokens) : "l"(plan_tokens + nx_g));
-          asm volatile("ld.global.nc.s32 %0, [%1];" : "=r"(nx_start) : "l"(plan_starts + nx_g));
+          asm volatile("ld.global.s32 %0, [%1];" : "=r"(nx_tokens) : "l"(plan_tokens + nx_g));
+          asm volatile("ld.global.s32 %0, [%1];" : "=r"(nx_start) : "l"(plan_starts + nx_g));
         }
       }
       ++nx_step;
@@ -463,7 +464,7 @@ k_grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
       float rs = 1.0f;
       const float* cs = nullptr;
       if constexpr (kFp8) {
-        rs = row_ok ? __ldg(a_scale + static_cast<long long>(g) * m_dim + row) : 0.f;
+        rs = row_ok ? a_scale[static_cast<long long>(g) * m_dim + row] : 0.f;
         cs = b_scale + static_cast<long long>(g) * n_dim;
       }
       const int row_w0 = mt * kBlockM + quarter * 32;

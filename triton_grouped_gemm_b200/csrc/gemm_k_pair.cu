@@ -51,8 +51,8 @@ template <bool kFp8>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNumThreads, 1)
 k_grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
                       const __grid_constant__ CUtensorMap tm_c, void* __restrict__ c_ptr, int num_groups, int m_dim,
-                      int n_dim, int in_fmt, int out_fp16, const float* __restrict__ a_scale,
-                      const float* __restrict__ b_scale, int* __restrict__ scratch, unsigned* status) {
+                      int n_dim, int in_fmt, int out_fp16, const float* a_scale,
+                      const float* b_scale, int* scratch, unsigned* status) {
   using L = KPairSmem;
   constexpr int kStages = kKPairStages;
   constexpr int kDepth = kKPairSchedDepth;
@@ -175,11 +175,11 @@ k_grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_con
       } else if (nx_step == 1) {
         nx_t = __shfl_sync(0xFFFFFFFFu, nx_t, 0);
         if (nx_t < num_tiles)
-          asm volatile("ld.global.nc.s32 %0, [%1];" : "=r"(nx_g) : "l"(plan_order + nx_t / tiles_per_group));
+          asm volatile("ld.global.s32 %0, [%1];" : "=r"(nx_g) : "l"(plan_order + nx_t / tiles_per_group));
       } else if (nx_step == 2) {
         if (nx_t < num_tiles) {
-          asm volatile("ld.global.nc.s32 %0, [%1];" : "=r"(nx_tokens) : "l"(plan_tokens + nx_g));
-          asm volatile("ld.global.nc.s32 %0, [%1];" : "=r"(nx_start) : "l"(plan_starts + nx_g));
+          asm volatile("ld.global.s32 %0, [%1];" : "=r"(nx_tokens) : "l"(plan_tokens + nx_g));
+          asm volatile("ld.global.s32 %0, [%1];" : "=r"(nx_start) : "l"(plan_starts + nx_g));
         }
       }
       ++nx_step;
@@ -371,7 +371,7 @@ k_grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_con
       float rs = 1.0f;
       const float* cs = nullptr;
       if constexpr (kFp8) {
-        rs = row_ok ? __ldg(a_scale + static_cast<long long>(g) * m_dim + row) : 0.f;
+        rs = row_ok ? a_scale[static_cast<long long>(g) * m_dim + row] : 0.f;
         cs = b_scale + static_cast<long long>(g) * n_dim;
       }
       if (row_w0 + 32 <= m_dim)

@@ -40,9 +40,9 @@ template <bool kBMnMajor, bool kFp8>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNumThreads, 1)
 m_grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
                       const __grid_constant__ CUtensorMap tm_c, void* __restrict__ c_ptr,
-                      const void* __restrict__ sizes, int sizes_i64, int num_groups, int masked_stride,
-                      long long m_rows, int n, int k, int in_fmt, int out_fp16, const float* __restrict__ a_scale,
-                      const float* __restrict__ b_scale, unsigned* status) {
+                      const void* sizes, int sizes_i64, int num_groups, int masked_stride,
+                      long long m_rows, int n, int k, int in_fmt, int out_fp16, const float* a_scale,
+                      const float* b_scale, unsigned* status) {
   static_assert(!(kFp8 && kBMnMajor), "fp8 operands are K-major only");
   using L = PairSmem;
   constexpr int kStages = kPairStages;
@@ -211,7 +211,7 @@ m_grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_con
       float rs = 1.0f;
       const float* cs = nullptr;
       if constexpr (kFp8) {
-        rs = row_ok ? __ldg(a_scale + row) : 0.f;
+        rs = row_ok ? a_scale[row] : 0.f;
         cs = b_scale + static_cast<long long>(w.g) * n;
       }
       if (row_w0 + 32 <= w.group_row_end())

@@ -31,7 +31,7 @@ __device__ __forceinline__ uint32_t pack2_16bit(float lo, float hi, int is_fp16)
 template <int kBlockN, bool kScaled>
 __device__ __forceinline__ void store_acc_row_16bit(uint32_t t_addr, uint16_t* c_row, bool row_ok, int col_base,
                                                     int n, int is_fp16, float row_scale = 1.0f,
-                                                    const float* __restrict__ col_scale = nullptr) {
+                                                    const float* col_scale = nullptr) {
 #pragma unroll 1
   for (int c = 0; c < kBlockN / 32; ++c) {
     uint32_t r[32];
@@ -46,8 +46,8 @@ __device__ __forceinline__ void store_acc_row_16bit(uint32_t t_addr, uint16_t* c
 #pragma unroll
           for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(r[v * 8 + e]);
           if constexpr (kScaled) {
-            const float4 s0 = __ldg(reinterpret_cast<const float4*>(col_scale + col0 + v * 8));
-            const float4 s1 = __ldg(reinterpret_cast<const float4*>(col_scale + col0 + v * 8 + 4));
+            const float4 s0 = *reinterpret_cast<const float4*>(col_scale + col0 + v * 8);
+            const float4 s1 = *reinterpret_cast<const float4*>(col_scale + col0 + v * 8 + 4);
             const float cs[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
 #pragma unroll
             for (int e = 0; e < 8; ++e) f[e] = __fmul_rn(__fmul_rn(f[e], row_scale), cs[e]);
@@ -74,7 +74,7 @@ template <int kBlockN, bool kScaled>
 __device__ __forceinline__ void store_acc_warp_tma(uint32_t t_addr, const CUtensorMap* tm_c, uint8_t* stage, int& sel,
                                                    int row_warp0, int z, int col_base, int n, int is_fp16, int lane,
                                                    float row_scale = 1.0f,
-                                                   const float* __restrict__ col_scale = nullptr) {
+                                                   const float* col_scale = nullptr) {
 #pragma unroll 1
   for (int c = 0; c < kBlockN / 64; ++c) {
     const int col0 = col_base + c * 64;
@@ -97,8 +97,8 @@ __device__ __forceinline__ void store_acc_warp_tma(uint32_t t_addr, const CUtens
       for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(r[v * 8 + e]);
       if constexpr (kScaled) {
         if (col0 + v * 8 < n) {
-          const float4 s0 = __ldg(reinterpret_cast<const float4*>(col_scale + col0 + v * 8));
-          const float4 s1 = __ldg(reinterpret_cast<const float4*>(col_scale + col0 + v * 8 + 4));
+          const float4 s0 = *reinterpret_cast<const float4*>(col_scale + col0 + v * 8);
+          const float4 s1 = *reinterpret_cast<const float4*>(col_scale + col0 + v * 8 + 4);
           const float cs[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
 #pragma unroll
           for (int e = 0; e < 8; ++e) f[e] = __fmul_rn(__fmul_rn(f[e], row_scale), cs[e]);

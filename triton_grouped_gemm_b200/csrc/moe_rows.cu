@@ -50,8 +50,8 @@ __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
 }
 
 // lane j < top_k: the row pair (t, j) owns, or -1 (and the status bit)
-__device__ __forceinline__ long long owned_row(const long long* __restrict__ pos, const long long* __restrict__ order,
-                                               long long t, int top_k, long long num_rows, int lane, unsigned* status) {
+__device__ __forceinline__ long long owned_row(const long long* pos, const long long* order, long long t,
+                                               int top_k, long long num_rows, int lane, unsigned* status) {
   long long r = -1;
   if (lane < top_k) {
     const long long p = t * top_k + lane;
@@ -67,9 +67,8 @@ __device__ __forceinline__ long long owned_row(const long long* __restrict__ pos
 // Zeros the rows of [first, first + count) that no pair owns (count <= 32).  vb0 / kStep: the warp's first vector
 // and its stride.
 template <int kStep>
-__device__ __forceinline__ void zero_unowned(uint4* __restrict__ dst, const long long* __restrict__ pos,
-                                             const long long* __restrict__ order, long long first, int count,
-                                             long long pairs, int row_vecs, int lane, int vb0) {
+__device__ __forceinline__ void zero_unowned(uint4* __restrict__ dst, const long long* pos, const long long* order,
+                                             long long first, int count, long long pairs, int row_vecs, int lane, int vb0) {
   bool unowned = false;
   if (lane < count) {
     const long long p = order[first + lane];
@@ -103,9 +102,8 @@ struct UnitWalk {
 
 template <bool kSpread>
 __global__ void __launch_bounds__(kRowsThreads)
-permute_rows_kernel(const uint4* __restrict__ x, const long long* __restrict__ pos, const long long* __restrict__ order,
-                    uint4* __restrict__ out, long long tokens, int top_k, int row_vecs, long long num_rows,
-                    long long units, unsigned* status) {
+permute_rows_kernel(const uint4* x, const long long* pos, const long long* order, uint4* __restrict__ out, long long tokens,
+                    int top_k, int row_vecs, long long num_rows, long long units, unsigned* status) {
   constexpr int kStep = UnitWalk<kSpread>::kStep;
   const UnitWalk<kSpread> w;
   chain_wait();
@@ -118,7 +116,7 @@ permute_rows_kernel(const uint4* __restrict__ x, const long long* __restrict__ p
         uint4 q[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (v + e * kStep < row_vecs) q[e] = __ldg(s + v + e * kStep);
+          if (v + e * kStep < row_vecs) q[e] = s[v + e * kStep];
         for (int j = 0; j < top_k; ++j) {
           const long long r = __shfl_sync(0xFFFFFFFFu, mine, j);
           if (r < 0) continue;
@@ -141,9 +139,9 @@ permute_rows_kernel(const uint4* __restrict__ x, const long long* __restrict__ p
 // fetched anew from the lanes that hold them.
 template <bool kSpread, int kK, int kU, bool kRounds, bool kFp16>
 __global__ void __launch_bounds__(kRowsThreads)
-combine_rows_kernel(const uint4* __restrict__ rows, const long long* __restrict__ pos,
-                    const long long* __restrict__ order, const float* __restrict__ weights, uint4* __restrict__ out,
-                    long long tokens, int top_k, int row_vecs, long long num_rows, unsigned* status) {
+combine_rows_kernel(const uint4* rows, const long long* pos, const long long* order, const float* weights,
+                    uint4* __restrict__ out, long long tokens, int top_k, int row_vecs, long long num_rows,
+                    unsigned* status) {
   constexpr int kStep = UnitWalk<kSpread>::kStep;
   const UnitWalk<kSpread> w;
   chain_wait();
@@ -175,7 +173,7 @@ combine_rows_kernel(const uint4* __restrict__ rows, const long long* __restrict_
         for (int i = 0; i < kU; ++i)
 #pragma unroll
           for (int j = 0; j < kK; ++j)
-            if (src[j] && v + i * kStep < row_vecs) q[i][j] = __ldg(src[j] + v + i * kStep);
+            if (src[j] && v + i * kStep < row_vecs) q[i][j] = src[j][v + i * kStep];
 #pragma unroll
         for (int i = 0; i < kU; ++i)
 #pragma unroll
@@ -199,9 +197,8 @@ combine_rows_kernel(const uint4* __restrict__ rows, const long long* __restrict_
 // compiler takes 145 registers, three blocks and 1000 us for the case above; 4, 5 and 6 blocks 926, 909 and 952 us.
 template <bool kSpread, int kK, bool kFp16>
 __global__ void __launch_bounds__(kRowsThreads, 5)
-combine_rows_grad_kernel(const uint4* __restrict__ dout, const uint4* __restrict__ rows,
-                         const long long* __restrict__ pos, const long long* __restrict__ order,
-                         const float* __restrict__ weights, uint4* __restrict__ drows, float* __restrict__ dweights,
+combine_rows_grad_kernel(const uint4* dout, const uint4* rows, const long long* pos, const long long* order,
+                         const float* weights, uint4* __restrict__ drows, float* __restrict__ dweights,
                          long long tokens, int top_k, int row_vecs, long long num_rows, long long units,
                          unsigned* status) {
   constexpr int kStep = UnitWalk<kSpread>::kStep;
@@ -224,12 +221,12 @@ combine_rows_grad_kernel(const uint4* __restrict__ dout, const uint4* __restrict
           dot[j] = 0.f;
         }
         for (int v = w.vb0 + w.lane; v < row_vecs; v += kStep) {
-          const uint4 qd = __ldg(dout + u * row_vecs + v);
+          const uint4 qd = dout[u * row_vecs + v];
           uint4 q[kK];
           if (dweights) {
 #pragma unroll
             for (int j = 0; j < kK; ++j)
-              if (r[j] >= 0) q[j] = __ldg(rows + r[j] * row_vecs + v);
+              if (r[j] >= 0) q[j] = rows[r[j] * row_vecs + v];
           }
           float d[8];
           unpack8<kFp16>(qd, d);

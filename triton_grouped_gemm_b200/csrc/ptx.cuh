@@ -411,4 +411,8 @@ __device__ __forceinline__ void cluster_sync_all() {
 __device__ __forceinline__ void chain_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void chain_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
+// What its predecessor may have written, such a kernel reads with ordinary loads (ld.global).  The predecessor still runs
+// while the kernel is resident, and ld.global.nc is for memory that nobody writes as long as the kernel lives: the compiler
+// takes it for __ldg and for pointers that are both const and __restrict__, so neither occurs.
+
 }  // namespace b200
