@@ -13,6 +13,7 @@ from ctypes import c_char_p, c_int, c_int64, c_void_p, c_uint, POINTER, c_float
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 import os
 
@@ -162,6 +163,43 @@ _no_guard = contextlib.nullcontext()
 def on_device(device: torch.device):
     """``with on_device(t.device):`` - a device guard that costs nothing where that device is current already."""
     return _no_guard if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
+
+
+_modes, _tracing, _grad_enabled = torch._C._len_torch_dispatch_stack, torch._C._is_tracing, torch.is_grad_enabled
+
+
+def _refuse_proxies(what: str) -> None:
+    from torch.fx.experimental.proxy_tensor import get_proxy_mode
+
+    if get_proxy_mode() is not None:
+        raise RuntimeError(f"{what} cannot be traced by make_fx: the kernel writes through a pointer, which the graph would lose")
+
+
+def recorded(what: str, *tensors: torch.Tensor) -> bool:
+    """Whether a call on ``tensors`` has to go through its ``torch.autograd.Function``: a gradient is wanted, a forward-mode
+    level is open, or ``torch.jit.trace`` records.  Called directly, the kernel would write a tensor that knows nothing of
+    the operands: tangents and traces would be lost without a word."""
+    if _modes():
+        _refuse_proxies(what)
+    if _tracing() or forward_ad._current_level >= 0:
+        return True
+    if _grad_enabled():
+        for t in tensors:
+            if t.requires_grad:
+                return True
+    return False
+
+
+def refuse_recorded_out(what: str, *tensors: torch.Tensor) -> None:
+    """``out=`` is written behind autograd's back: no gradient, and refused where that would go unnoticed."""
+    if _modes():
+        _refuse_proxies(what)
+    if _tracing():
+        raise RuntimeError(f"{what} with out= cannot be traced")
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{what} with out= has no forward-mode derivative")
 
 
 def ptr(t: torch.Tensor) -> int:

@@ -101,7 +101,7 @@ def permute_rows(x: torch.Tensor, pos: torch.Tensor, order: torch.Tensor, top_k:
     assert x.dim() == 2, "x must be 2D [T, H]"
     _check_plan("permute_rows", x, pos, order, x.shape[0] * top_k)
     x = x.contiguous()
-    if x.requires_grad and torch.is_grad_enabled():
+    if _lib.recorded("permute_rows", x):
         return _PermuteRows.apply(x, pos, order, top_k)
     return _permute(x, pos, order, top_k)
 
@@ -115,7 +115,7 @@ def combine_rows(rows: torch.Tensor, topk_weight: torch.Tensor, pos: torch.Tenso
     _check_plan("combine_rows", rows, pos, order, topk_weight.numel())
     assert topk_weight.get_device() == rows.get_device(), "combine_rows: all operands must be on one device"
     rows = rows.contiguous()
-    if (rows.requires_grad or topk_weight.requires_grad) and torch.is_grad_enabled():
+    if _lib.recorded("combine_rows", rows, topk_weight):
         return _CombineRows.apply(rows, topk_weight, pos, order)
     t, top_k = topk_weight.shape
     return _combine(rows, topk_weight.to(torch.float32).contiguous(), pos, order, t, top_k)

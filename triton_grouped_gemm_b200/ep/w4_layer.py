@@ -25,7 +25,7 @@ class W4MoELayer:
     @torch.no_grad()
     def forward(self, x: torch.Tensor, topk_idx: torch.Tensor, topk_weight: torch.Tensor) -> torch.Tensor:
         """x [T, H] of the weights' type, topk_idx / topk_weight [T, k] -> [T, H].  A pair whose expert id is out of
-        range is dropped."""
+        range is dropped.  Runs under ``no_grad``: the result is detached."""
         plan = make_plan(topk_idx, self.num_experts)
         rows = permute_rows(x, plan.pos, plan.send_order, plan.top_k)
         h = m_grouped_gemm_w4_gated(rows, self.w13, plan.size_per_group, self.activation)

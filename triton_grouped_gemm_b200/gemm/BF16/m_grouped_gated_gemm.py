@@ -91,10 +91,25 @@ def _m_grouped_gated_grad_launch(dY: Tensor, W2: Tensor, saved: Tensor, exps: Te
     return dgu
 
 
+class _MGroupedGatedGemm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, A, B, size_per_group, activation, masked_stride, numSM):
+        return _m_grouped_gated_launch(A, B, size_per_group, activation, masked_stride=masked_stride, numSM=numSM)[0]
+
+    @staticmethod
+    def backward(ctx, dh):
+        raise RuntimeError("m_grouped_gated_gemm has no gradient; grouped_gated_ffn is the block with one")
+
+
 def m_grouped_gated_gemm(A: Tensor, B: Tensor, size_per_group: Tensor, activation: str = "silu", *,
                          masked_stride: int = 0, out: Optional[Tensor] = None, numSM: int = -1) -> Tensor:
     """[M, I] of A [M, K], B [G, 2*I, K] (gate rows, then up rows); ``activation`` "silu" or "gelu_tanh".
     K and I are multiples of 8.  ``masked_stride`` > 0: masked row layout (``masked_stride`` rows per group, the
     first ``size_per_group[g]`` of them valid).  Rows outside the groups are left as they were in ``out``.  No
-    gradient: see ``gemm.autograd.grouped_gated_ffn``."""
+    gradient (differentiating through the result raises; ``out`` is written outside autograd): see
+    ``gemm.autograd.grouped_gated_ffn``."""
+    if out is not None:
+        _lib.refuse_recorded_out("m_grouped_gated_gemm", A, B)
+    elif _lib.recorded("m_grouped_gated_gemm", A, B):
+        return _MGroupedGatedGemm.apply(A, B, size_per_group, activation, masked_stride, numSM)
     return _m_grouped_gated_launch(A, B, size_per_group, activation, out=out, masked_stride=masked_stride, numSM=numSM)[0]

@@ -163,6 +163,6 @@ def grouped_gated_ffn(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, size
     x, w13, w2 = x.contiguous(), w13.contiguous(), w2.contiguous()
     if size_per_group.dtype not in (torch.int32, torch.int64):
         size_per_group = size_per_group.to(torch.int64)
-    if torch.is_grad_enabled() and (x.requires_grad or w13.requires_grad or w2.requires_grad):
+    if _lib.recorded("grouped_gated_ffn", x, w13, w2):
         return _GroupedGatedFfn.apply(x, w13, w2, size_per_group, activation)
     return _gated_ffn_forward(x, w13, w2, size_per_group, activation, save=False)[3]
