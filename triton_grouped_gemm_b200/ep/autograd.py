@@ -121,13 +121,20 @@ def combine_rows(rows: torch.Tensor, topk_weight: torch.Tensor, pos: torch.Tenso
     return _combine(rows, topk_weight.to(torch.float32).contiguous(), pos, order, t, top_k)
 
 
+def check_routing(what: str, x: torch.Tensor, topk_idx: torch.Tensor, topk_weight: torch.Tensor) -> None:
+    assert x.dim() == 2 and topk_idx.dim() == 2 and topk_idx.shape[0] == x.shape[0], \
+        f"{what}: x must be 2D [T, H] and topk_idx 2D [T, k]"
+    assert topk_weight.shape == topk_idx.shape, f"{what}: topk_weight must have topk_idx's shape"
+
+
 def moe_ffn(x: torch.Tensor, topk_idx: torch.Tensor, topk_weight: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor,
             activation: str = "silu") -> torch.Tensor:
     """Trainable 16-bit MoE feed-forward layer on one rank: x [T, H], topk_idx [T, k] (an id outside the experts drops
     the pair), topk_weight [T, k], w13 [E, 2*I, H] (gate rows, then up rows), w2 [E, H, I] -> [T, H], with gradients
-    for x, topk_weight, w13 and w2.  Nothing synchronises the host.  The plan leaves the order of the rows inside an
+    for x, topk_weight, w13 and w2.  Nothing synchronises the host (up to 1024 experts).  The plan leaves the order of the rows inside an
     expert open: it changes nothing in the output or the gradients of x and topk_weight, but the weights' gradients sum
     over the rows and may differ in their last bits from one call to the next."""
+    check_routing("moe_ffn", x, topk_idx, topk_weight)
     top_k = topk_idx.shape[1]
     plan = make_plan(topk_idx, w13.shape[0])
     rows = permute_rows(x, plan.pos, plan.send_order, top_k)

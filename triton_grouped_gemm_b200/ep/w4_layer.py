@@ -7,7 +7,7 @@ import torch
 
 from ..gemm.W4.m_grouped_gemm_w4 import m_grouped_gemm_w4, m_grouped_gemm_w4_gated
 from ..quant.per_group_cast import per_group_cast_to_w4
-from .autograd import combine_rows, permute_rows
+from .autograd import check_routing, combine_rows, permute_rows
 from .dispatch import make_plan
 
 
@@ -26,6 +26,7 @@ class W4MoELayer:
     def forward(self, x: torch.Tensor, topk_idx: torch.Tensor, topk_weight: torch.Tensor) -> torch.Tensor:
         """x [T, H] of the weights' type, topk_idx / topk_weight [T, k] -> [T, H].  A pair whose expert id is out of
         range is dropped.  Runs under ``no_grad``: the result is detached."""
+        check_routing("W4MoELayer", x, topk_idx, topk_weight)
         plan = make_plan(topk_idx, self.num_experts)
         rows = permute_rows(x, plan.pos, plan.send_order, plan.top_k)
         h = m_grouped_gemm_w4_gated(rows, self.w13, plan.size_per_group, self.activation)
