@@ -174,7 +174,7 @@ int b200gemm_m_grouped_gated_grad(const void* dy, const void* w2, const void* sa
  *   c[r, n] = sum_grp scale[g, n, grp] * sum_{k in grp} (q[g, n, k] - zero[g, n, grp]) * a[r, k]
  * fp32 accumulate, one rounding.  a [m_rows, k] compact rows (bf16 / fp16); w4 [G, N, k/2] bytes, element 2j
  * in the low and 2j+1 in the high half of byte j; scale [G, N, k/group_size] of a's type; zero
- * [G, N, k/group_size] bytes (0..15) or NULL (8 everywhere); group_size 32, 64 or 128, k a multiple of it.
+ * [G, N, k/group_size] bytes (0..15, not checked) or NULL (8 everywhere); group_size 32, 64 or 128, k a multiple of it.
  *   gated == 0: N = n, out [m_rows, n] = c.
  *   gated != 0: N = 2 n (gate rows, then up rows), out = act(c_gate) * c_up (act as above).
  * sizes as for b200gemm_m_grouped (cut off at m_rows); at most 1024 groups; n is free of alignment.

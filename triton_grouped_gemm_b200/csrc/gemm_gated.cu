@@ -20,7 +20,7 @@
 //     issuer, two accumulators, epilogue warps that store through swizzled staging buffers.
 //
 // Measured with 655 360 rows over 128 groups, K 2048, I 768, beside the plain M-grouped product of the same shape on
-// the same GPU: forward 2.78 ms (2.72), keeping g and u 3.26 ms (3.38 - the same, both at the power limit), gradient
+// the same GPU: forward 2.78 ms (2.72), keeping g and u 3.26 ms, gradient
 // 1.94 ms (1.66; it reads 2.0 GB and writes 2.0 GB where the plain product writes 1.0 GB).  With integer arithmetic for
 // the codes and an exactly rounded reciprocal they took 3.96 and 3.54 ms: the epilogue, not the tensor cores, was the
 // bound, and it still is in fp16 layers: keeping g and u 3.8-4.2 ms, gradient 2.2-2.5 ms (gelu 4.0 and 2.7; bf16 layers

@@ -6,7 +6,9 @@
 // weights' bytes, N * K / 2 per expert that has a row; the arithmetic only has to keep up with them:
 //
 //   * a 4-bit value becomes a 16-bit one by OR-ing it into the mantissa of a power of two (128 + q in bf16,
-//     1024 + q in fp16) and subtracting 128 + zero (1024 + zero): exact, 1.4 instructions per value (fp16: 1.1).
+//     1024 + q in fp16) and subtracting 128 + zero (1024 + zero): exact, 1.4 instructions per value (fp16: 1.1).  The
+//     method is published: Kim, Henry, Fahim, Awadalla, "Who Says Elephants Can't Run: Bringing Large Scale MoE Models into
+//     Cloud Scale Production", 2022; the constants follow from the two number formats.
 //   * products run on mma.sync m16n8k16 with the WEIGHTS as the 16-row operand and up to 8 rows of `a` as the
 //     8 columns.  tcgen05 wants the weights in 16 bits in shared memory (four times the bytes that bound this kernel)
 //     or in tensor memory.  The latter was built - 128 weight rows unpacked into tensor memory by two warpgroups,
@@ -117,7 +119,8 @@ __device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t m
   return r;
 }
 
-// magic + zero in both halves: 0x43zz is 128 + zz in bf16 (zz < 128), 0x64zz is 1024 + zz in fp16
+// magic + zero in both halves: 0x43zz is 128 + zz in bf16 (zz < 128), 0x64zz is 1024 + zz in fp16.  Zeros are 0 .. 15 by
+// contract; beyond 127 the bf16 sum would need a ninth bit.
 template <bool kFp16>
 __device__ __forceinline__ uint32_t zero_pair(uint32_t zero) {
   return ((kFp16 ? 0x6400u : 0x4300u) + zero) * 0x10001u;
@@ -584,10 +587,12 @@ w4_m_grouped_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
 }
 
 // ------------------------------------------------------------------ quantiser
-// One warp per 32 * kPer-element group: min / max by shuffles, then every lane packs kPer values.  Symmetric:
+// 16 lanes per group of 16 * kPer elements: min / max by shuffles, then every lane packs kPer values.  Symmetric:
 // scale = max|w| / 7, q = clamp(round(w / scale) + 8).  Asymmetric: scale = (max(w,0) - min(w,0)) / 15,
 // zero = round(-min / scale), q = clamp(round(w / scale) + zero).  Scales are rounded to the weights' type first and
-// that rounded scale is what the values are divided by; a group of zeros has scale 0.  Bound by HBM bytes; run once.
+// that rounded scale is what the values are divided by; a group of zeros has scale 0.  Run once per weight tensor: 2-byte
+// loads and a correctly rounded division per value bound it, far from the bytes (128 x 1536 x 2048 bf16, 1.0 GB: groups of
+// 128 483 us, 2.1 TB/s; of 32 with zeros 889 us, 1.2 TB/s).
 template <int kPer, bool kFp16>
 __global__ void __launch_bounds__(256)
 w4_quant_kernel(const uint16_t* __restrict__ w, uint8_t* __restrict__ q, uint16_t* __restrict__ scale,

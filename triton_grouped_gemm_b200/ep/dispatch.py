@@ -7,7 +7,7 @@ the row layout the grouped GEMMs consume (``size_per_group`` = rows per local ex
 ``dispatch`` moves row payloads (any dtype, e.g. fp8 bytes and their fp32 scales) to the
 owning ranks; ``combine`` brings per-row results back and sums the top-k contributions of a
 token with the router weights.  The only collectives are all_to_all_single calls; on GPUs the
-process group is NCCL, in the CPU tests it is gloo.
+process group is NCCL, in the CPU tests it is gloo.  ``ep.autograd`` has the 16-bit movers of one rank, with gradients.
 """
 
 from __future__ import annotations

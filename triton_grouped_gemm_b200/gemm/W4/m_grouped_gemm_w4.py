@@ -5,7 +5,8 @@ Weights are what ``quant.per_group_cast.per_group_cast_to_w4`` produces:
     b = (w4 [G, N, K/2] uint8, scale [G, N, K/group_size], zero [G, N, K/group_size] uint8 or None)
     C[r, n] = sum_grp scale[g, n, grp] * sum_{k in grp} (q[g, n, k] - zero[g, n, grp]) * a[r, k]
 
-Element 2j of a row is the low half of byte j, element 2j+1 the high half; ``zero=None`` stands for 8 everywhere;
+Element 2j of a row is the low half of byte j, element 2j+1 the high half; a ``zero`` is a whole number 0..15 (not
+checked: beyond 15 bf16 and fp16 need not agree), ``zero=None`` stands for 8 everywhere;
 ``scale`` has the type of ``a`` (bf16 or fp16).  The reference has no 4-bit path.
 """
 
